@@ -584,6 +584,40 @@ gd_status gd_linear_sum_assignment(const float* cost, int problems, int Q, int K
                                    gd_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Optimizer step over many tensors (csrc/optim.hip)                         */
+/* ------------------------------------------------------------------------ */
+/*
+ * One AdamW update (decoupled weight decay) of `tensors` tensors:
+ *   g  = grad * min(1, max_norm / (*total_norm + 1e-6))   (total_norm not NULL)
+ *   m' = beta1 m + (1 - beta1) g,  v' = beta2 v + (1 - beta2) g^2
+ *   p' = p (1 - lr weight_decay)
+ *        - lr / (1 - beta1^t) m' / (sqrt(v') / sqrt(1 - beta2^t) + eps)
+ * The lists are HOST arrays of `tensors` device addresses, numel their element
+ * counts (tensors of no elements are skipped); tensors are contiguous, of any
+ * alignment of their element, and do not overlap.
+ * params fp32, grads grad_dtype (fp32 / bf16); copies NULL, or bf16 tensors
+ * that receive the new weights rounded.
+ * state_bits 32: exp_avgs, exp_avg_sqs fp32, the scales NULL.
+ * state_bits 8: per 32 consecutive elements one scale byte s (2^(s - 127), s in
+ * 0..254, a fresh state zero everywhere) and e4m3 values; exp_avgs holds m,
+ * exp_avg_sqs holds sqrt(v).  Rounded stochastically by a counter-based number
+ * of (seed, t, element).  Scale lists: ceil(numel / 32) bytes each.
+ * t: `step` (from 1), or per tensor a device fp32 count in steps_dev; lr_dev
+ * (device fp32) replaces lr when not NULL.  No host copy or synchronisation: the
+ * call can be captured into a graph. */
+gd_status gd_adamw_step(int tensors, const int64_t* numel, const uint64_t* params, int grad_dtype,
+                        const uint64_t* grads, int state_bits, const uint64_t* exp_avgs, const uint64_t* exp_avg_sqs,
+                        const uint64_t* exp_avg_scales, const uint64_t* exp_avg_sq_scales, const uint64_t* copies,
+                        const uint64_t* steps_dev, double step, double lr, const float* lr_dev, double beta1,
+                        double beta2, double eps, double weight_decay, const float* total_norm, double max_norm,
+                        uint32_t seed, gd_stream_t stream);
+/* out[0] = sqrt(sum of the squares of all elements), squared and summed in
+ * double in a fixed order.  workspace: gd_grad_norm_workspace_bytes. */
+size_t gd_grad_norm_workspace_bytes(int tensors, const int64_t* numel);
+gd_status gd_grad_norm(int tensors, const int64_t* numel, int dtype, const uint64_t* grads, void* workspace,
+                       size_t workspace_bytes, float* out, gd_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Runtime                                                                   */
 /* ------------------------------------------------------------------------ */
 const char* gd_last_error(void);

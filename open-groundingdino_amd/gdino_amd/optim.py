@@ -1,0 +1,332 @@
+"""AdamW over many tensors and the gradient norm on MI355X (csrc/optim.hip).
+
+``grad_norm(grads)``        2-norm over all gradients, summed in double
+``adamw_step(params, ...)`` one AdamW update of a list of tensors, with the
+                            clip by that norm folded in
+``AdamW``                   the same as a torch.optim.Optimizer
+
+A model's step is a handful of launches whatever its number of tensors, and
+the clip costs one read of the gradients: they are scaled as the update reads
+them, and keep their unclipped values.  The moments are fp32, or 8 bits: e4m3
+values times a power of two per 32 consecutive elements, stochastically rounded,
+of the first moment and of the ROOT of the second (csrc/optim.hip says why).
+Weights are fp32; a low-precision model keeps fp32 masters, and the step writes
+its bf16 weights beside them.
+
+The reference trains with torch.optim.AdamW and clip_grad_norm_ (main.py:254-292,
+engine_multi.py:562-564); ``train.build_optimizer`` picks this optimizer
+with ``args.optimizer = "adamw_hip"`` (``args.optimizer_state_bits`` 32 or 8).
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+_p, _i, _f64, _u32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_uint32
+_lib.register("gd_adamw_step", [_i, _p, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, _f64, _f64, _p, _f64, _f64, _f64,
+                                _f64, _p, _f64, _u32, _p])
+_lib.register("gd_grad_norm", [_i, _p, _i, _p, _p, ctypes.c_size_t, _p, _p])
+
+BLOCK = 32  # elements of an 8-bit moment that share a scale
+_GRAD_TYPES = (_lib.GD_F32, _lib.GD_BF16)
+_U8, _E4M3, _E8M0 = 4, 5, 6  # _tensors.TYPES
+
+
+def _describe(tensors, written=False):
+    from . import _tensors  # built beside the library (csrc/Makefile)
+    return _tensors.describe(tensors if type(tensors) is list else list(tensors), written)
+
+
+def _guard(device: int):
+    """The launches go to the tensors' device, also where another is current."""
+    if device >= 0 and device != torch.cuda.current_device():
+        return torch.cuda.device(device)
+    return contextlib.nullcontext()
+
+
+def _check(what, name, got, n, device, types, sizes=None):
+    """One list's description against the call's: its length, place, layout, type and element counts."""
+    addr, size, kind, dev, dense = got
+    if len(addr) != 8 * n:
+        raise ValueError(f"{what}: {len(addr) // 8} {name} for {n} tensors")
+    if n and dev != device:
+        raise RuntimeError(f"{what}: {name} are not all on the device of the first tensor")
+    if not dense:
+        raise RuntimeError(f"{name} tensors have to be contiguous ({what})")
+    if n and kind not in types:
+        raise TypeError(f"gdino_amd {what}: unsupported or mixed dtypes of {name}")
+    if sizes is not None and size != sizes:
+        raise ValueError(f"{what}: {name} and the weights differ in their numbers of elements")
+    return addr
+
+
+def _scalar(what, name, t, device):
+    """The address of a one-element fp32 tensor on the call's device."""
+    if t.dtype != torch.float32 or t.numel() != 1:
+        raise TypeError(f"gdino_amd {what}: {name} is a one-element fp32 tensor, not {t.dtype} {tuple(t.shape)}")
+    if _describe([t])[3] != device:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, the tensors are elsewhere")
+    return t.data_ptr()
+
+
+def grad_norm(grads) -> torch.Tensor:
+    """sqrt of the sum of all squares of ``grads`` (contiguous, all fp32 or
+    all bf16, on one device) -> 0-dim fp32 tensor.  No host synchronisation."""
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(())
+    what = "grad_norm"
+    got = _describe(grads)
+    device = got[3]
+    _lib.require_device(grads[0], what=what)
+    addr = _check(what, "gradients", got, len(grads), device, _GRAD_TYPES)
+    fn = _lib.lib().gd_grad_norm_workspace_bytes
+    fn.restype, fn.argtypes = ctypes.c_size_t, [_i, _p]
+    nbytes = int(fn(len(grads), got[1]))
+    with _guard(device):
+        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=grads[0].device)
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        _lib.call("gd_grad_norm", len(grads), got[1], got[2], addr, ws.data_ptr(), nbytes, out.data_ptr(),
+                  _lib.stream_of(out), nbytes=_elements(got) * (4 if got[2] == _lib.GD_F32 else 2))
+    return out
+
+
+def _elements(got):
+    return sum(memoryview(got[1]).cast("q")) if _lib.call_timer is not None else 0
+
+
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
+               exp_avg_scales=None, exp_avg_sq_scales=None, copies=None, total_norm=None, max_norm=0.0, seed=0) -> None:
+    """One AdamW update, in place, of the fp32 tensors ``params``:
+
+      g  = grad * min(1, max_norm / (total_norm + 1e-6))      (total_norm given)
+      m' = b1 m + (1 - b1) g,   v' = b2 v + (1 - b2) g^2
+      p' = p (1 - lr weight_decay) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+
+    grads: all fp32 or all bf16.  exp_avgs / exp_avg_sqs: fp32 m and v, or, with
+    ``exp_avg_scales`` and ``exp_avg_sq_scales`` (one byte per BLOCK elements, 2^(byte - 127)), m and sqrt(v) as
+    e4m3 bytes (``adamw_state`` makes either).  step: t, counted from 1, or a
+    list of one-element fp32 device tensors that hold it (they are read, not
+    advanced).  lr: a number or a one-element fp32 device tensor.  copies: bf16
+    tensors that receive the new weights.  total_norm: ``grad_norm``'s result.
+    seed: of the 8-bit moments' stochastic rounding.
+
+    Tensors are contiguous, of any alignment, on one device; those of a list
+    that is written must not overlap.  No host synchronisation: with the step
+    counts and lr on the device the call can be captured and replayed."""
+    what = "adamw_step"
+    params = list(params)
+    n = len(params)
+    got = _describe(params, True)
+    device = got[3]
+    if n:
+        _lib.require_device(params[0], what=what)
+    pa = _check(what, "weights", got, n, device, (_lib.GD_F32,))
+    sizes = got[1]
+    g = _describe(grads)
+    ga = _check(what, "gradients", g, n, device, _GRAD_TYPES, sizes)
+    eight = exp_avg_scales is not None
+    if eight != (exp_avg_sq_scales is not None):
+        raise ValueError(f"{what}: moments in 8 bits have two lists of scales")
+    kinds = (_U8, _E4M3) if eight else (_lib.GD_F32,)
+    ma = _check(what, "exp_avgs", _describe(exp_avgs, True), n, device, kinds, sizes)
+    va = _check(what, "exp_avg_sqs", _describe(exp_avg_sqs, True), n, device, kinds, sizes)
+    msa = vsa = ca = sa = None
+    if eight:
+        blocks = memoryview(sizes).cast("q")
+        blocks = (ctypes.c_int64 * n)(*[-(-k // BLOCK) for k in blocks])
+        msa, vsa = (_check(what, name, _describe(x, True), n, device, (_U8, _E8M0), bytes(blocks))
+                    for name, x in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)))
+    if copies is not None:
+        ca = _check(what, "copies", _describe(copies, True), n, device, (_lib.GD_BF16,), sizes)
+    if isinstance(step, (list, tuple)):
+        steps = _describe(step)
+        sa = _check(what, "steps", steps, n, device, (_lib.GD_F32,))
+        if any(k != 1 for k in memoryview(steps[1]).cast("q")):
+            raise ValueError(f"{what}: a step count is one element")
+        step = 0
+    elif not step >= 1:
+        raise ValueError(f"{what}: step counts from 1, not {step}")
+    b1, b2 = (float(b) for b in betas)
+    if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
+        raise ValueError(f"{what}: betas {betas}, eps {eps}, weight_decay {weight_decay}")
+    lr_dev = None
+    if torch.is_tensor(lr) and not lr.is_cpu:
+        lr_dev, lr = _scalar(what, "lr", lr, device), 0.0
+    lr = float(lr)
+    if not (lr >= 0.0 and math.isfinite(lr)):
+        raise ValueError(f"{what}: lr {lr}")
+    norm = None
+    if total_norm is not None:
+        if not max_norm > 0.0:
+            raise ValueError(f"{what}: total_norm comes with a positive max_norm")
+        norm = _scalar(what, "total_norm", total_norm, device)
+    if n == 0:
+        return
+    with _guard(device):
+        _lib.call("gd_adamw_step", n, sizes, pa, g[2], ga, 8 if eight else 32, ma, va, msa, vsa, ca, sa, float(step),
+                  lr, lr_dev, b1, b2, float(eps), float(weight_decay), norm, float(max_norm), int(seed) & 0xFFFFFFFF,
+                  _lib.stream_of(params[0]),
+                  nbytes=_elements(got) * (8 + (4 if g[2] == _lib.GD_F32 else 2) + (4.125 if eight else 16)
+                                           + (0 if ca is None else 2)))
+    torch.autograd.graph.increment_version(params)
+    if copies is not None:
+        torch.autograd.graph.increment_version(copies)
+
+
+def adamw_state(p: torch.Tensor, bits: int = 32) -> dict:
+    """Fresh (zero) moments of ``p``: {"exp_avg", "exp_avg_sq"}, in 8 bits also
+    {"exp_avg_scale", "exp_avg_sq_scale"} (``adamw_step``'s lists hold these)."""
+    if bits == 32:
+        return {k: torch.zeros_like(p, dtype=torch.float32, requires_grad=False, memory_format=torch.preserve_format)
+                for k in ("exp_avg", "exp_avg_sq")}
+    if bits != 8:
+        raise ValueError(f"moments have 32 or 8 bits, not {bits}")
+    out = {}
+    for k in ("exp_avg", "exp_avg_sq"):
+        out[k] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+        out[k + "_scale"] = torch.zeros(-(-p.numel() // BLOCK), dtype=torch.uint8, device=p.device)
+    return out
+
+
+def state_value(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The fp32 values an 8-bit moment stands for (of exp_avg_sq: the root)."""
+    x = codes.reshape(-1).view(torch.float8_e4m3fn).float()
+    s = torch.exp2(scales.view(torch.uint8).double() - 127).float()
+    return (x * s.repeat_interleave(BLOCK)[:x.numel()]).view(codes.shape)
+
+
+def _memory_order(p: torch.Tensor):
+    """The permutation of p's dimensions that makes it contiguous."""
+    order = sorted(range(p.dim()), key=lambda d: (-p.stride(d), d))
+    if not p.permute(order).is_contiguous():
+        raise ValueError(f"AdamW: weights are dense in memory; strides {p.stride()} of {tuple(p.shape)} are not")
+    return order
+
+
+class AdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW's update on csrc/optim.hip.
+
+    state_bits: 32, or 8 for moments of 8 bits (2.06 bytes per weight instead
+    of 8).  Weights in bf16 get an fp32 master in their state, which the update
+    reads and writes; the weights are its rounding.  The step counts live
+    on the device, ``lr`` may be a device tensor: a step can be captured.
+    With 32 bits the state is torch.optim.AdamW's, and either loads the other's.
+
+    step(max_norm=...) clips the gradients by their norm over all groups as
+    clip_grad_norm_ does, without writing them; the norm stays in
+    ``total_norm``."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits {state_bits}: 8 or 32")
+        if not (float(lr) >= 0.0 and 0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0
+                and weight_decay >= 0.0):
+            raise ValueError(f"AdamW: lr {lr}, betas {betas}, eps {eps}, weight_decay {weight_decay}")
+        # capturable: what torch's loader asks before it moves a step count to the device
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      seed=seed, capturable=True))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dtype not in (torch.float32, torch.bfloat16):
+                    raise TypeError(f"gdino_amd AdamW: unsupported dtype {p.dtype}")
+        self.total_norm = None
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("total_norm", None)
+
+    def _state(self, p, bits):
+        st = self.state[p]
+        if not st:
+            if bits == 8 and not p.is_contiguous():
+                raise ValueError("AdamW: 8-bit moments belong to contiguous weights (their scales go by memory)")
+            st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            st.update(adamw_state(p, bits))
+            if p.dtype != torch.float32:
+                st["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+        return st
+
+    def _lists(self, group):
+        """{(weight type, gradient type, device): {"param": [...], "grad": [...], the state's keys}}."""
+        lists = {}
+        for p in group["params"]:
+            g = p.grad
+            if g is None:
+                continue
+            if g.is_sparse:
+                raise RuntimeError("AdamW: sparse gradients are not supported")
+            row = {"param": p, "grad": g, **self._state(p, group["state_bits"])}
+            if not p.is_contiguous():  # (a channels_last weight: everything is walked in its memory's order)
+                order = _memory_order(p)
+                row = {k: t.detach().permute(order) if t.shape == p.shape and k != "step" else t
+                       for k, t in row.items()}
+            if not row["grad"].is_contiguous():
+                row["grad"] = row["grad"].contiguous()
+            into = lists.setdefault((p.dtype, g.dtype, p.device), {k: [] for k in row})
+            for k, t in row.items():
+                into[k].append(t)
+        return lists
+
+    @torch.no_grad()
+    def step(self, closure=None, max_norm: float = 0.0):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = [(group, key, row) for group in self.param_groups for key, row in self._lists(group).items()]
+        self.total_norm = norm = self._norm(work) if max_norm > 0.0 and work else None
+        for group, _, row in work:
+            torch._foreach_add_(row["step"], 1)
+            masters = row.get("master")
+            adamw_step(row["param"] if masters is None else masters, row["grad"], row["exp_avg"], row["exp_avg_sq"],
+                       row["step"], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], exp_avg_scales=row.get("exp_avg_scale"),
+                       exp_avg_sq_scales=row.get("exp_avg_sq_scale"),
+                       copies=None if masters is None else row["param"], total_norm=norm, max_norm=max_norm,
+                       seed=group["seed"])
+        return loss
+
+    def _norm(self, work):
+        by_type = {}
+        for _, (_, gdtype, dev), row in work:
+            by_type.setdefault((gdtype, dev), []).extend(row["grad"])
+        if len({dev for _, dev in by_type}) > 1:
+            raise RuntimeError("AdamW: the norm of gradients on several devices; clip them before the step")
+        norms = [grad_norm(g) for g in by_type.values()]
+        # (fp32 and bf16 gradients side by side: the norm of the norms)
+        return norms[0] if len(norms) == 1 else grad_norm(norms)
+
+    def load_state_dict(self, state_dict):
+        bits = [g["state_bits"] for g in self.param_groups]
+        seeds = [g["seed"] for g in self.param_groups]
+        saved, at = {}, 0
+        flat = [p for g in self.param_groups for p in g["params"]]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        if len(flat) == len(ids):
+            for p, i in zip(flat, ids):
+                saved[p] = state_dict["state"].get(i, {})
+        want = {p: b for g, b in zip(self.param_groups, bits) for p in g["params"]}
+        for p, st in saved.items():
+            if "exp_avg" in st and (st["exp_avg"].dtype == torch.uint8) != (want[p] == 8):
+                raise ValueError(f"AdamW: the saved moments are not of {want[p]} bits")
+        super().load_state_dict(state_dict)
+        for g, b, s in zip(self.param_groups, bits, seeds):
+            g["state_bits"], g["capturable"] = b, True
+            g.setdefault("seed", s)
+        for p, st in saved.items():
+            # (torch's loader casts a state to its weight's type: bytes and masters keep theirs; moments are fp32)
+            for k, v in st.items():
+                if k == "step":
+                    self.state[p][k] = torch.as_tensor(v, dtype=torch.float32).to(p.device).clone()
+                elif torch.is_tensor(v):
+                    dt = torch.float32 if v.is_floating_point() else v.dtype
+                    like = p if v.shape == p.shape else v
+                    self.state[p][k] = torch.empty_like(like, dtype=dt, device=p.device, requires_grad=False).copy_(v)
+            if st and p.dtype != torch.float32 and "master" not in st:
+                self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)

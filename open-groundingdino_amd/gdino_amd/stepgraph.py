@@ -60,7 +60,7 @@ import torch.distributed as dist
 
 from . import _lib, castcache
 from .misc import bump_mask_epoch, local_only, no_padding
-from .train import BucketedGradSync, weighted_loss
+from .train import BucketedGradSync, clip_and_step, weighted_loss
 
 _VERBOSE = os.environ.get("GDINO_STEPGRAPH_VERBOSE") == "1"
 # A/B knobs: the capture's error mode and the cache's shared memory pool
@@ -286,9 +286,7 @@ class TrainStepGraph:
         loss.backward()
         if self.grad_sync is not None:
             self.grad_sync.after_backward()
-        if self.clip_max_norm > 0:
-            torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.clip_max_norm, foreach=True)
-        self.optimizer.step()
+        clip_and_step(self.model.parameters(), self.optimizer, self.clip_max_norm)
         return loss.detach(), {k: v.detach() for k, v in loss_dict.items()}
 
     def _stream_ctx(self):
@@ -354,6 +352,8 @@ class TrainStepGraph:
                     if torch.is_tensor(v):
                         if old is not None and k in old:
                             v.copy_(old[k])
+                        elif k == "master":  # (optim.AdamW: a low-precision weight's fp32 master)
+                            v.copy_(p)
                         else:
                             v.zero_()
                     elif old is not None and k in old:

@@ -18,6 +18,7 @@ from typing import List, Tuple
 
 import torch
 
+from . import optim
 from .misc import NestedTensor, collectives_enabled
 
 
@@ -129,7 +130,16 @@ def get_param_dict(args, model):
 
 
 def build_optimizer(args, model):
+    """AdamW over the parameter groups.  args.optimizer: "adamw" (default,
+    torch's) or "adamw_hip" (gdino_amd.optim.AdamW, the clip folded into the
+    update; args.optimizer_state_bits 32 or 8)."""
     groups = [g for g in get_param_dict(args, model) if g["params"]]
+    kind = getattr(args, "optimizer", "adamw")
+    if kind == "adamw_hip":
+        return optim.AdamW(groups, lr=args.lr, weight_decay=args.weight_decay,
+                           state_bits=getattr(args, "optimizer_state_bits", 32))
+    if kind != "adamw":
+        raise ValueError(f"optimizer {kind} not supported")
     # fused AdamW: one multi-tensor launch chain instead of per-parameter ops
     return torch.optim.AdamW(groups, lr=args.lr, weight_decay=args.weight_decay,
                              fused=next(model.parameters()).is_cuda)
@@ -159,6 +169,17 @@ def weighted_loss(loss_dict, weight_dict):
             _LOSS_WEIGHTS.clear()
         w = _LOSS_WEIGHTS[ck] = torch.tensor(ck[1], dtype=dt).to(dev)
     return (torch.stack(vals) * w).sum()
+
+
+def clip_and_step(parameters, optimizer, clip_max_norm: float):
+    """clip_grad_norm_(parameters, clip_max_norm), then optimizer.step(); an
+    optim.AdamW does both over its own parameters, leaving .grad unclipped."""
+    if isinstance(optimizer, optim.AdamW):
+        optimizer.step(max_norm=clip_max_norm)
+        return
+    if clip_max_norm > 0:
+        torch.nn.utils.clip_grad_norm_(parameters, clip_max_norm, foreach=True)
+    optimizer.step()
 
 
 class GradAllReduce:
@@ -407,9 +428,7 @@ def train_step(model, criterion, optimizer, samples, targets, captions, cat_list
         grad_sync.after_backward()
     elif grad_sync is not None:
         grad_sync()
-    if clip_max_norm > 0:
-        torch.nn.utils.clip_grad_norm_(model.parameters(), clip_max_norm, foreach=True)
-    optimizer.step()
+    clip_and_step(model.parameters(), optimizer, clip_max_norm)
     return loss.detach()
 
 

@@ -337,6 +337,37 @@ inline float fdot2_bf16(V2 a, V2 b, float c) {
   return float(double(float(a[0])) * double(float(b[0])) + double(float(a[1])) * double(float(b[1])) + double(c));
 }
 
+// v_cvt_pk_f32_fp8 / v_cvt_pk_fp8_f32 (OCP e4m3: 4 exponent bits of bias 7, 3
+// mantissa bits, 0x7F NaN, no infinity): two values of the low or high half word
+inline float e4m3_to_f(uint8_t b) {
+  const int e = (b >> 3) & 15, m = b & 7;
+  const float v = (b & 0x7F) == 0x7F ? NAN : (e ? ldexpf(float(8 + m), e - 10) : ldexpf(float(m), -9));
+  return b & 0x80 ? -v : v;
+}
+inline uint8_t f_to_e4m3(float f) {  // nearest, ties to even; saturates
+  const uint8_t sign = std::signbit(f) ? 0x80 : 0;
+  const float a = fabsf(f);
+  if (!(a == a)) return 0x7F;
+  int best = 0;
+  for (int i = 1; i < 0x7F; ++i) {
+    const float d = fabsf(e4m3_to_f(uint8_t(i)) - a), b = fabsf(e4m3_to_f(uint8_t(best)) - a);
+    if (d < b || (d == b && !(i & 1))) best = i;
+  }
+  return uint8_t(sign | best);
+}
+typedef float gd_emu_f32x2 __attribute__((ext_vector_type(2)));
+inline gd_emu_f32x2 cvt_pk_f32_fp8(int w, bool hi) {
+  const unsigned u = unsigned(w) >> (hi ? 16 : 0);
+  gd_emu_f32x2 r;
+  r[0] = e4m3_to_f(uint8_t(u));
+  r[1] = e4m3_to_f(uint8_t(u >> 8));
+  return r;
+}
+inline int cvt_pk_fp8_f32(float a, float b, int old, bool hi) {
+  const unsigned h = f_to_e4m3(a) | unsigned(f_to_e4m3(b)) << 8, o = unsigned(old);
+  return int(hi ? (o & 0xFFFFu) | h << 16 : (o & 0xFFFF0000u) | h);
+}
+
 template <typename V8, typename C4>
 inline C4 mfma_16x16x32_bf16(V8 a, V8 b, C4 c) {
   static_assert(sizeof(V8) == 16 && sizeof(C4) == 16, "bf16x8 / f32x4 operands");
@@ -423,6 +454,8 @@ inline int __ffsll(long long v) { return __builtin_ffsll(v); }
 #define __builtin_amdgcn_mov_dpp(src, ctrl, rm, bm, bc) ::gd_emu::update_dpp((src), (src), (ctrl), (rm), (bm), (bc))
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, cbsz, abid, blgp) \
   ::gd_emu::mfma_16x16x32_bf16((a), (b), (c))
+#define __builtin_amdgcn_cvt_pk_f32_fp8(w, hi) ::gd_emu::cvt_pk_f32_fp8((w), (hi))
+#define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) ::gd_emu::cvt_pk_fp8_f32((a), (b), (old), (hi))
 #define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) ::gd_emu::fdot2_bf16((a), (b), (c))
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) ::gd_emu::mfma_16x16x4_f32((a), (b), (c))
 #define hipLaunchKernelGGL(kernel, g, b, shm, stream, ...) \

@@ -1,0 +1,276 @@
+"""gdino_amd.optim without a GPU: the kernels' sources in the emulator (tests/emu), refusals, and the wiring."""
+import copy
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import emu_product
+import optim_cases as oc
+
+SIZES = [1, 3, 32, 33, 0, 4096, 4097, 1000]
+
+
+@pytest.fixture
+def emulated():
+    with emu_product.emulated_product():
+        yield
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("grad", [torch.float32, torch.bfloat16])
+def test_adamw_step(emulated, grad, offset):
+    from gdino_amd import optim
+    p, g, m, v = oc.make(SIZES, grad, offset=offset)
+    want = [oc.reference(*x, 4, **oc.HYPER) for x in zip(p, g, m, v)]
+    copies = [torch.zeros_like(x, dtype=torch.bfloat16) for x in p]
+    optim.adamw_step(p, g, m, v, 4, copies=copies, **oc.HYPER)
+    for got, (w, scale) in zip(zip(p, m, v), want):
+        oc.check_update(got, w, scale)
+    for a, b in zip(p, copies):
+        assert torch.equal(a.bfloat16(), b)
+
+
+def test_adamw_many_tensors_share_launches(emulated):
+    """More tensors than a launch's table holds (96), each with its own device step count."""
+    from gdino_amd import optim
+    sizes = [(7 * i) % 61 for i in range(230)]
+    p, g, m, v = oc.make(sizes)
+    steps = [torch.tensor(float(1 + i % 5)) for i in range(230)]
+    want = [oc.reference(*x, 1 + i % 5, **oc.HYPER) for i, x in enumerate(zip(p, g, m, v))]
+    lr = oc.HYPER | {"lr": torch.tensor(oc.HYPER["lr"])}
+    optim.adamw_step(p, g, m, v, steps, **lr)
+    for got, (w, scale) in zip(zip(p, m, v), want):
+        oc.check_update(got, w, scale)
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+def test_adamw_eight_bits(emulated, offset):
+    from gdino_amd import optim
+    p, g, m, v = oc.make([1, 31, 33, 4100], seed=3, offset=offset)
+    states = [optim.adamw_state(x, 8) for x in p]
+    lists = {k: [s[k] for s in states] for k in states[0]}
+    for t in (1, 2, 3):
+        before = [(oc.values(s["exp_avg"], s["exp_avg_scale"]), oc.values(s["exp_avg_sq"], s["exp_avg_sq_scale"]))
+                  for s in states]
+        want = [oc.reference(x, y, torch.from_numpy(a), torch.from_numpy(b ** 2), t, **oc.HYPER)
+                for x, y, (a, b) in zip(p, g, before)]
+        optim.adamw_step(p, g, lists["exp_avg"], lists["exp_avg_sq"], t, exp_avg_scales=lists["exp_avg_scale"],
+                         exp_avg_sq_scales=lists["exp_avg_sq_scale"], seed=11, **oc.HYPER)
+        for x, s, ((wp, wm, wv), (pa, ms, ua)) in zip(p, states, want):
+            assert ((x.double() - wp).abs() <= 4 * oc.U * pa + 24 * oc.U * ua).all()
+            u, w = oc.chance(x.numel(), 11, t)
+            oc.check_eight(s["exp_avg"], s["exp_avg_scale"], wm.numpy(), u, False)
+            oc.check_eight(s["exp_avg_sq"], s["exp_avg_sq_scale"], wv.sqrt().numpy(), w, True)
+
+
+def test_adamw_eight_bits_of_values_that_are_not_finite(emulated):
+    """An infinite or NaN gradient spoils its own element, not the others of its block."""
+    from gdino_amd import optim
+    p, g, _, _ = oc.make([64])
+    g[0][5], g[0][40] = math.inf, math.nan
+    s = optim.adamw_state(p[0], 8)
+    q = copy.deepcopy(p)
+    clean = [g[0].nan_to_num(0, 0, 0)]
+    r = optim.adamw_state(p[0], 8)
+    for w, x, st in ((p, g, s), (q, clean, r)):
+        optim.adamw_step(w, x, [st["exp_avg"]], [st["exp_avg_sq"]], 1, exp_avg_scales=[st["exp_avg_scale"]],
+                         exp_avg_sq_scales=[st["exp_avg_sq_scale"]], **oc.HYPER)
+    bad = torch.zeros(64, dtype=torch.bool)
+    bad[[5, 40]] = True
+    assert torch.equal(p[0][~bad], q[0][~bad]) and not torch.isfinite(p[0][bad]).any()
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert torch.equal(s[k][~bad], r[k][~bad]) and torch.isnan(optim.state_value(s[k], s[k + "_scale"])[bad]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_grad_norm_and_clip(emulated, dtype):
+    from gdino_amd import optim
+    p, g, m, v = oc.make(SIZES, dtype, seed=5)
+    exact = math.sqrt(sum(float(x.double().square().sum()) for x in g))
+    norm = optim.grad_norm(g)
+    assert abs(float(norm) - exact) <= 2 * oc.U * exact  # the sum is in double: the result's rounding
+    clip = 0.5 / (exact + 1e-6)
+    assert clip < 1
+    want = [oc.reference(*x, 2, clip=clip, **oc.HYPER) for x in zip(p, g, m, v)]
+    kept = [x.clone() for x in g]
+    optim.adamw_step(p, g, m, v, 2, total_norm=norm, max_norm=0.5, **oc.HYPER)
+    for got, (w, scale) in zip(zip(p, m, v), want):
+        oc.check_update(got, w, scale, clipped=True)
+    assert all(torch.equal(a, b) for a, b in zip(g, kept))
+
+
+def test_grad_norm_range(emulated):
+    """Squares beyond fp32's range, zeros, nothing, NaN."""
+    from gdino_amd import optim
+    assert float(optim.grad_norm([torch.full((3,), 1e30)])) == pytest.approx(math.sqrt(3) * 1e30, rel=1e-6)
+    assert float(optim.grad_norm([torch.full((4,), 1e-30)])) == pytest.approx(2e-30, rel=1e-6)
+    assert float(optim.grad_norm([torch.zeros(5), torch.zeros(0)])) == 0
+    assert float(optim.grad_norm([torch.zeros(0)])) == 0 and float(optim.grad_norm([])) == 0
+    assert math.isnan(float(optim.grad_norm([torch.tensor([1.0, math.nan])])))
+    assert math.isinf(float(optim.grad_norm([torch.tensor([1.0, -math.inf])])))
+
+
+def test_refusals(emulated):
+    from gdino_amd import _lib, optim
+
+    def step(p, g, m, v, t=1, **kw):
+        optim.adamw_step(p, g, m, v, t, **(oc.HYPER | kw))
+
+    p, g, m, v = oc.make([8, 8])
+    with pytest.raises(ValueError, match="overlap"):
+        step([p[0], p[0]], g, m, v)
+    with pytest.raises(ValueError, match="overlap"):
+        step(p, g, [m[0], m[0]], v)
+    with pytest.raises(ValueError, match="1 gradients for 2"):
+        step(p, g[:1], m, v)
+    with pytest.raises(ValueError, match="numbers of elements"):
+        step(p, [g[0], g[1][:7]], m, v)
+    with pytest.raises(TypeError, match="dtypes of gradients"):
+        step(p, [g[0], g[1].bfloat16()], m, v)
+    with pytest.raises(TypeError, match="dtypes of gradients"):
+        step(p, [x.half() for x in g], m, v)
+    with pytest.raises(TypeError, match="dtypes of weights"):
+        step([x.bfloat16() for x in p], g, m, v)
+    with pytest.raises(TypeError, match="not a tensor"):
+        step(p, [g[0], None], m, v)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        step([x.view(2, 4).t() for x in p], g, m, v)
+    with pytest.raises(ValueError, match="two lists of scales"):
+        step(p, g, m, v, exp_avg_scales=[])
+    with pytest.raises(ValueError, match="counts from 1"):
+        step(p, g, m, v, 0)
+    with pytest.raises(ValueError, match="lr"):
+        step(p, g, m, v, lr=-1.0)
+    with pytest.raises(ValueError, match="lr"):
+        step(p, g, m, v, lr=math.nan)
+    with pytest.raises(ValueError, match="betas"):
+        step(p, g, m, v, betas=(1.0, 0.9))
+    with pytest.raises(ValueError, match="max_norm"):
+        step(p, g, m, v, total_norm=torch.ones(()))
+    with pytest.raises(TypeError, match="one-element"):
+        step(p, g, m, v, total_norm=torch.ones(2), max_norm=1.0)
+    eight = [optim.adamw_state(x, 8) for x in p]
+    with pytest.raises(ValueError, match="exp_avg_scales"):
+        step(p, g, [s["exp_avg"] for s in eight], [s["exp_avg_sq"] for s in eight],
+             exp_avg_scales=[torch.zeros(2, dtype=torch.uint8), eight[1]["exp_avg_scale"]],
+             exp_avg_sq_scales=[s["exp_avg_sq_scale"] for s in eight])
+    with pytest.raises(TypeError, match="dtypes of gradients"):
+        optim.grad_norm([torch.zeros(3, dtype=torch.float64)])
+    with pytest.raises(ValueError):
+        optim.adamw_state(p[0], 16)
+    step([], [], [], [])
+    with pytest.raises(_lib.GdError, match="workspace"):
+        sizes = np.array([8], dtype=np.int64)
+        addr = np.array([p[0].data_ptr()], dtype=np.uint64)
+        _lib.call("gd_grad_norm", 1, sizes.tobytes(), 0, addr.tobytes(), None, 0, p[1].data_ptr(), None)
+
+
+def test_cpu_tensors_raise():
+    from gdino_amd import optim
+    p, g, m, v = oc.make([8])
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        optim.adamw_step(p, g, m, v, 1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        optim.grad_norm(g)
+
+
+def _model(dtype=torch.float32):
+    torch.manual_seed(1)
+    net = torch.nn.Sequential(torch.nn.Linear(5, 7), torch.nn.ReLU(), torch.nn.Linear(7, 3)).to(dtype)
+    net.add_module("conv", torch.nn.Conv2d(3, 4, 3).to(dtype))
+    net.conv.weight.data = net.conv.weight.data.contiguous(memory_format=torch.channels_last)
+    return net
+
+
+def _grads(net, seed):
+    g = torch.Generator().manual_seed(seed)
+    for i, p in enumerate(net.parameters()):
+        p.grad = None if i == 1 and seed == 2 else torch.randn(p.shape, generator=g).to(p.dtype)
+
+
+def test_optimizer_follows_torch(emulated):
+    """Three steps beside torch.optim.AdamW with clip_grad_norm_, a parameter without a gradient in one of them, a
+    channels_last weight; the checkpoint moves both ways."""
+    from gdino_amd import optim
+    ours, theirs = _model(), _model()
+    kw = dict(lr=1e-2, weight_decay=0.1)
+    a, b = optim.AdamW(ours.parameters(), **kw), torch.optim.AdamW(theirs.parameters(), **kw)
+
+    def step(seed):
+        for net in (ours, theirs):
+            _grads(net, seed)
+        a.step(max_norm=0.3)
+        norm = torch.nn.utils.clip_grad_norm_(theirs.parameters(), 0.3)
+        b.step()
+        torch.testing.assert_close(a.total_norm, norm)
+        for x, y in zip(ours.parameters(), theirs.parameters()):
+            torch.testing.assert_close(x, y, rtol=2e-6, atol=2e-6)
+
+    for seed in (1, 2, 3):
+        step(seed)
+    steps = [int(s["step"]) for s in a.state_dict()["state"].values()]
+    assert steps == [3, 2, 3, 3, 3, 3]
+    sa, sb = copy.deepcopy(a.state_dict()), copy.deepcopy(b.state_dict())
+    a.load_state_dict(sb)
+    b.load_state_dict({"state": sa["state"], "param_groups": sb["param_groups"]})
+    step(4)
+
+
+def test_optimizer_eight_bits_and_masters(emulated):
+    from gdino_amd import optim
+    net = _model(torch.bfloat16)
+    net.conv.weight.data = net.conv.weight.data.contiguous()
+    opt = optim.AdamW(net.parameters(), lr=1e-3, state_bits=8)
+    for seed in (1, 2):
+        _grads(net, seed)
+        opt.step()
+    for p in net.parameters():
+        st = opt.state[p]
+        assert st["exp_avg"].dtype == torch.uint8 and st["master"].dtype == torch.float32
+        assert torch.equal(st["master"].bfloat16(), p)
+    saved = copy.deepcopy(opt.state_dict())
+    again = optim.AdamW(_model(torch.bfloat16).parameters(), lr=1e-3, state_bits=8)
+    again.load_state_dict(saved)
+    for s, q in zip(saved["state"].values(), again.param_groups[0]["params"]):
+        for k, x in s.items():
+            assert torch.equal(again.state[q][k], x) and again.state[q][k].dtype == x.dtype
+    with pytest.raises(ValueError, match="32 bits"):
+        optim.AdamW(net.parameters(), lr=1e-3).load_state_dict(saved)
+
+
+def test_optimizer_refusals(emulated):
+    from gdino_amd import optim
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        optim.AdamW([torch.zeros(3, dtype=torch.float64, requires_grad=True)])
+    with pytest.raises(ValueError, match="state_bits"):
+        optim.AdamW([torch.zeros(3, requires_grad=True)], state_bits=4)
+    p = torch.zeros(4, 4)[:, :2].requires_grad_()
+    p.grad = torch.ones_like(p)
+    with pytest.raises(ValueError, match="dense"):
+        optim.AdamW([p]).step()
+    q = torch.zeros(2, 3, 4, 4).contiguous(memory_format=torch.channels_last).requires_grad_()
+    q.grad = torch.ones_like(q)
+    with pytest.raises(ValueError, match="contiguous weights"):
+        optim.AdamW([q], state_bits=8).step()
+
+
+def test_train_step_uses_it(emulated):
+    """build_optimizer picks the optimizer by args, clip_and_step folds the clip into it."""
+    from gdino_amd import castcache, optim, train
+    from gdino_amd.config import make_args
+    net = _model()
+    args = make_args(device="cpu", param_dict_type="default", optimizer="adamw_hip", optimizer_state_bits=32)
+    opt = train.build_optimizer(args, net)
+    assert isinstance(opt, optim.AdamW)
+    assert isinstance(train.build_optimizer(make_args(device="cpu", param_dict_type="default"), net),
+                      torch.optim.AdamW)
+    with pytest.raises(ValueError, match="not supported"):
+        train.build_optimizer(make_args(device="cpu", param_dict_type="default", optimizer="sgd"), net)
+    _grads(net, 1)
+    kept = [p.grad.clone() for p in net.parameters()]
+    versions, generation = [p._version for p in net.parameters()], castcache._generation
+    train.clip_and_step(net.parameters(), opt, 0.1)
+    assert all(torch.equal(p.grad, k) for p, k in zip(net.parameters(), kept))
+    assert all(p._version > v for p, v in zip(net.parameters(), versions)) and castcache._generation == generation + 1
