@@ -1,0 +1,797 @@
+// A linear layer with its epilogue, and its gradients, for gfx950:
+//
+//   z = x W^T + b     y = act(z) + r          x [M, K], W [N, K], bf16 / fp16
+//   dz = dy * act'(z)     dx = dz W     dW = dz^T x     db = sum_m dz     (dr = dy)
+//
+// All three products are one kernel, C[m][n] = sum_r A(m, r) B(n, r), whose
+// operands lie in memory either with r contiguous ("rows": x, W, dz in the
+// forward and dx) or with m / n contiguous ("columns": W in dx, dz and x in dW).
+// Products of 16-bit values are exact in fp32 and the accumulators are fp32
+// matrix-core registers; bias, activation and residual are applied to them in
+// fp32 and the result is rounded once.  The backward rounds dz to 16 bits, as the
+// matrix instructions take it, and needs act'(z): the forward writes z rounded to
+// 16 bits beside y (for ReLU without a residual y itself tells where z > 0).
+//
+// Where the output has too few tiles to fill 256 CUs the sum over r is split: the
+// parts go to a workspace in fp32 and a finishing kernel adds them in a fixed
+// order and applies the epilogue.  There are no atomics: results repeat bit
+// by bit.
+#include "gd_common.h"
+
+#include <cmath>
+
+namespace gd {
+namespace {
+
+enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4 };
+
+typedef short gd_i16x8 __attribute__((ext_vector_type(8)));
+typedef short gd_i16x4 __attribute__((ext_vector_type(4)));
+typedef float gd_f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 gd_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
+
+// the two 16-bit types
+struct Bf16 {
+  static __device__ __forceinline__ float up(uint16_t h) { return bf16_to_f32(h); }
+  static __device__ __forceinline__ uint16_t down(float f) { return f32_to_bf16(f); }
+  static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b),
+                                                   c, 0, 0, 0);
+  }
+};
+struct Fp16 {
+  static __device__ __forceinline__ float up(uint16_t h) { return float(__builtin_bit_cast(_Float16, h)); }
+  static __device__ __forceinline__ uint16_t down(float f) {
+    const _Float16 h = (_Float16)f;
+    return __builtin_bit_cast(uint16_t, h);
+  }
+  static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gd_f16x8, a), __builtin_bit_cast(gd_f16x8, b), c,
+                                                  0, 0, 0);
+  }
+};
+
+// ---- activations ------------------------------------------------------------
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+
+// The normal distribution's Phi(z), and exp(-z^2 / 2) for its density: Abramowitz and Stegun 7.1.26,
+// erfc(x) = t (a1 + t (a2 + ...)) exp(-x^2), t = 1 / (1 + p x), off by 1.5e-7 at most; on -|z|, so that the tail
+// keeps its sign and does not cancel.
+__device__ __forceinline__ float normal_cdf(float z, float* bell) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * x);
+  const float e = exp_of(-0.5f * z * z);
+  const float q = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * q * e;
+  *bell = e;
+  return z > 0.f ? 1.f - tail : (z <= 0.f ? tail : z);
+}
+
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_of(-z)); }
+
+constexpr float kTanhC = 0.79788456080286536f, kTanhA = 0.044715f;
+
+// (the switch around the 8 values: a uniform branch each, not eight)
+__device__ __forceinline__ void activate8(float v[8], int act) {
+  switch (act) {
+    case kRelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];  // (NaN stays)
+      break;
+    case kGelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float bell;
+        v[j] *= normal_cdf(v[j], &bell);
+      }
+      break;
+    case kGeluTanh:  // (1 + tanh u) / 2 = sigmoid(2 u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= sigmoid(2.f * kTanhC * (v[j] + kTanhA * v[j] * v[j] * v[j]));
+      break;
+    case kSilu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= sigmoid(v[j]);
+      break;
+    default: break;
+  }
+}
+
+// d[j] *= act'(z[j])
+__device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
+  switch (act) {
+    case kRelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = z[j] > 0.f ? d[j] : 0.f;
+      break;
+    case kGelu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float bell;
+        const float c = normal_cdf(z[j], &bell);
+        d[j] *= c + z[j] * bell * 0.39894228040143268f;
+      }
+      break;
+    case kGeluTanh:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float q = sigmoid(2.f * kTanhC * (z[j] + kTanhA * z[j] * z[j] * z[j]));
+        d[j] *= q + 2.f * z[j] * q * (1.f - q) * kTanhC * (1.f + 3.f * kTanhA * z[j] * z[j]);
+      }
+      break;
+    case kSilu:
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float q = sigmoid(z[j]);
+        d[j] *= q * (1.f + z[j] * (1.f - q));
+      }
+      break;
+    default: break;
+  }
+}
+
+// ---- 8 consecutive 16-bit or fp32 values, the first `left` of them valid ------
+template <typename E>
+__device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool vec, int left, float v[8]) {
+  if (f32) {
+    const float* q = static_cast<const float*>(p) + at;
+    if (vec && left >= 8) {
+      const float4 a = reinterpret_cast<const float4*>(q)[0], b = reinterpret_cast<const float4*>(q)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < left ? q[j] : 0.f;
+    }
+    return;
+  }
+  const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+  union {
+    uint4 u;
+    uint16_t h[8];
+  } w;
+  if (vec && left >= 8) {
+    w.u = *reinterpret_cast<const uint4*>(q);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w.h[j] = j < left ? q[j] : uint16_t(0);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = E::up(w.h[j]);
+}
+
+template <typename E>
+__device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int left, const float v[8]) {
+  if (f32) {
+    float* q = static_cast<float*>(p) + at;
+    if (vec && left >= 8) {
+      reinterpret_cast<float4*>(q)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(q)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) q[j] = v[j];
+    }
+    return;
+  }
+  uint16_t* q = static_cast<uint16_t*>(p) + at;
+  union {
+    uint4 u;
+    uint16_t h[8];
+  } w;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
+  if (vec && left >= 8) {
+    *reinterpret_cast<uint4*>(q) = w.u;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < left) q[j] = w.h[j];
+  }
+}
+
+// ---- the epilogue -------------------------------------------------------------
+struct Epi {
+  const uint16_t* bias;  // or NULL
+  const void* res;       // or NULL
+  void* y;
+  uint16_t* z;           // or NULL: z for the backward, its rows padded to 8 with zeros
+  int64_t ldr, ldy, ldz;
+  int act;
+  bool bias_vec, res_f32, res_vec, y_f32, y_vec;
+};
+
+template <typename E>
+__device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N, float v[8]) {
+  const int left = N - n < 8 ? N - n : 8;
+  if (e.bias) {
+    float b[8];
+    ld8<E>(e.bias, n, false, e.bias_vec, left, b);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += b[j];
+  }
+  if (e.z) {
+    float z[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = j < left ? v[j] : 0.f;
+    st8<E>(e.z, m * e.ldz + n, false, true, 8, z);
+  }
+  activate8(v, e.act);
+  if (e.res) {
+    float r[8];
+    ld8<E>(e.res, m * e.ldr + n, e.res_f32, e.res_vec, left, r);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += r[j];
+  }
+  st8<E>(e.y, m * e.ldy + n, e.y_f32, e.y_vec, left, v);
+}
+
+// ---- the product ----------------------------------------------------------------
+struct Gemm {
+  const uint16_t *a, *b;  // 16-byte aligned, row pitches multiples of 8
+  int64_t lda, ldb;
+  int M, N;      // the output
+  int ra, rb;    // extents of r in memory; the shorter operand counts as zero beyond (rows: multiples of 8)
+  int ca, cb;    // columns in memory of a "columns" operand, multiples of 8
+  int splits, r_per_split;  // r_per_split: a multiple of kR
+  int tiles_n;
+  float* part;   // splits > 1: [splits][M][N]
+  Epi epi;
+};
+
+constexpr int kR = 64;  // values of r per staged chunk
+
+// Offset of 16-byte chunk ch of row r in an LDS image.  Rows image [x][64 r]: 128-byte rows; 16 lanes read the same
+// chunk of 16 consecutive rows, so the chunk index is xored with row / 2: with the row's parity that is every one of
+// the 16 positions of 256 bytes, all 64 banks.
+__device__ __forceinline__ int row_at(int row, int ch) { return row * kR + ((ch ^ ((row >> 1) & 7)) << 3); }
+// Columns image [64 r][X]: the transposing read (ds_read_b64_tr_b16) of half a wave touches rows q and 8 + q, q < 4, 32
+// bytes each, which have to lie 32 bytes apart modulo 256.
+template <int X>
+__device__ __forceinline__ int col_at(int r, int ch) {
+  const int swz = X == 64 ? 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1) : 2 * (r & 3) + 8 * ((r >> 3) & 1);
+  return r * X + ((ch ^ swz) << 3);
+}
+
+__device__ __forceinline__ gd_i16x4 lds_tr(const uint16_t* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gd_i16x4*)(p));
+}
+
+// the operand of one 16 x 16 x 32 product: lane (c, g) holds r = 8 g .. 8 g + 7 of row x0 + c, chunk s of 32
+template <int X, bool COL>
+__device__ __forceinline__ gd_i16x8 fragment(const uint16_t* img, int x0, int s, int lane) {
+  if constexpr (!COL) {
+    return *reinterpret_cast<const gd_i16x8*>(img + row_at(x0 + (lane & 15), 4 * s + (lane >> 4)));
+  } else {
+    const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
+    const int ch = (x0 >> 3) + (p >> 1), sub = 4 * (p & 1);
+    const gd_i16x4 lo = lds_tr(img + col_at<X>(32 * s + 8 * g + q, ch) + sub);
+    const gd_i16x4 hi = lds_tr(img + col_at<X>(32 * s + 8 * g + 4 + q, ch) + sub);
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+// WM x WN waves, each of TM x TN blocks of 16 x 16
+template <typename E, int WM, int WN, int TM, int TN, bool AC, bool BC>
+__global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
+  constexpr int kThreads = 64 * WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
+  constexpr int kStage = (BM + BN) * kR, NA = BM * 8 / kThreads, NB = BN * 8 / kThreads;
+  constexpr int kPitch = 16 * TN + 4;  // floats: the epilogue's rows
+  static_assert(WM * WN * 16 * kPitch * 2 <= 2 * kStage, "the epilogue's staging fits");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStage];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  // the tiles of one part of r, n fastest, contiguous per XCD: they share rows of A and all of B in its L2
+  const int L = xcd_remap(int(blockIdx.x), int(gridDim.x));
+  const int tiles = int(gridDim.x) / p.splits;
+  const int split = L / tiles, tile = L - split * tiles;
+  const int m0 = tile / p.tiles_n * BM, n0 = tile % p.tiles_n * BN;
+  const int r_end = p.ra > p.rb ? p.ra : p.rb;
+  const int rb0 = split * p.r_per_split;
+  const int re = rb0 + p.r_per_split < r_end ? rb0 + p.r_per_split : r_end;
+
+  uint4 ra[NA], rb[NB];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int h = 0; h < NA; ++h) {
+      const int v = tid + kThreads * h;
+      const int x = AC ? m0 + 8 * (v % (BM / 8)) : m0 + (v >> 3), r = r0 + (AC ? v / (BM / 8) : 8 * (v & 7));
+      const bool ok = r < p.ra && x < (AC ? p.ca : p.M);
+      ra[h] = ok ? *reinterpret_cast<const uint4*>(p.a + (AC ? r * p.lda + x : x * p.lda + r)) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      const int v = tid + kThreads * h;
+      const int x = BC ? n0 + 8 * (v % (BN / 8)) : n0 + (v >> 3), r = r0 + (BC ? v / (BN / 8) : 8 * (v & 7));
+      const bool ok = r < p.rb && x < (BC ? p.cb : p.N);
+      rb[h] = ok ? *reinterpret_cast<const uint4*>(p.b + (BC ? r * p.ldb + x : x * p.ldb + r)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  auto stash = [&](uint16_t* img) {
+#pragma unroll
+    for (int h = 0; h < NA; ++h) {
+      const int v = tid + kThreads * h;
+      *reinterpret_cast<uint4*>(img + (AC ? col_at<BM>(v / (BM / 8), v % (BM / 8)) : row_at(v >> 3, v & 7))) = ra[h];
+    }
+#pragma unroll
+    for (int h = 0; h < NB; ++h) {
+      const int v = tid + kThreads * h;
+      *reinterpret_cast<uint4*>(img + BM * kR + (BC ? col_at<BN>(v / (BN / 8), v % (BN / 8)) : row_at(v >> 3, v & 7))) =
+          rb[h];
+    }
+  };
+
+  gd_f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = gd_f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (rb0 < re) load(rb0);
+  for (int r0 = rb0, buf = 0; r0 < re; r0 += kR, buf ^= 1) {
+    uint16_t* img = lds + buf * kStage;
+    stash(img);
+    if (r0 + kR < re) load(r0 + kR);  // in flight during the products
+    gd_lds_barrier();                 // image complete; the other one was consumed an iteration ago
+#pragma unroll
+    for (int s = 0; s < kR / 32; ++s) {
+      gd_i16x8 fa[TM], fb[TN];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = fragment<BM, AC>(img, 16 * (wm * TM + i), s, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = fragment<BN, BC>(img + BM * kR, 16 * (wn * TN + j), s, lane);
+      // transposed: lane (c, g) receives C[16 i + c][16 j + 4 g .. + 3], four values of a row
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = E::mma(fb[j], fa[i], acc[i][j]);
+    }
+  }
+
+  // Each wave passes 16 rows at a time through its own LDS, so that a row leaves in 16-byte pieces of neighbouring
+  // lanes; pitch 16 TN + 4: 16 rows' float4s, and the reads of 8 neighbouring columns, touch all banks once.
+  __syncthreads();
+  float* own = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
+  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes;  // lanes per row, rows per pass
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      *reinterpret_cast<gd_f32x4*>(own + (lane & 15) * kPitch + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+    gd_wave_sync();
+#pragma unroll
+    for (int h = 0; h < 16 / kRows; ++h) {
+      const int row = h * kRows + lane / kLanes, col = 8 * (lane % kLanes);
+      const int m = m0 + 16 * (wm * TM + i) + row, n = n0 + 16 * wn * TN + col;
+      const float4 u = *reinterpret_cast<const float4*>(own + row * kPitch + col);
+      const float4 w = *reinterpret_cast<const float4*>(own + row * kPitch + col + 4);
+      float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+      if (m < p.M && n < p.N) {
+        if (p.splits > 1)
+          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, p.N - n, v);
+        else
+          epilogue8<E>(p.epi, m, n, p.N, v);
+      }
+    }
+    gd_wave_sync();
+  }
+}
+
+// the parts added in order, then the epilogue; a thread per 8 columns
+template <typename E>
+__global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ part, int splits, int M, int N, Epi epi) {
+  const int per_row = (N + 7) / 8;
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= int64_t(M) * per_row) return;
+  const int64_t m = i / per_row;
+  const int n = int(i - m * per_row) * 8;
+  const bool vec = (N & 3) == 0;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    float u[8];
+    ld8<E>(part, (int64_t(s) * M + m) * N + n, true, vec, N - n, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] += u[j];
+  }
+  epilogue8<E>(epi, m, n, N, v);
+}
+
+// ---- dz = dy * act'(z), and parts of its column sums -------------------------------
+struct Dact {
+  const void* dy;
+  const uint16_t* z;  // NULL: no activation
+  uint16_t* dz;       // or NULL; rows padded to 8 with zeros
+  float* sums;        // or NULL: [workgroups][N]
+  int64_t lddy, ldz, lddz, rows;  // rows: of one workgroup
+  int M, N, act, lanes;           // lanes: of a row, a power of two up to 64
+  bool dy_f32, dy_vec, z_vec;
+};
+
+template <typename E>
+__global__ void __launch_bounds__(256) linear_dact(const Dact p) {
+  __shared__ float lds[256 * 9];
+  const int slab = 8 * p.lanes, at = threadIdx.x / p.lanes, rows = 256 / p.lanes;
+  const int n = int(blockIdx.y) * slab + 8 * (threadIdx.x % p.lanes);
+  const int64_t begin = int64_t(blockIdx.x) * p.rows;
+  const int64_t end = begin + p.rows < p.M ? begin + p.rows : p.M;
+  const int left = p.N - n < 8 ? p.N - n : 8;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (left > 0) {
+#pragma unroll 2
+    for (int64_t m = begin + at; m < end; m += rows) {
+      float d[8];
+      ld8<E>(p.dy, m * p.lddy + n, p.dy_f32, p.dy_vec, left, d);
+      if (p.z) {
+        float z[8];
+        ld8<E>(p.z, m * p.ldz + n, false, p.z_vec, left, z);
+        slope8(d, z, p.act);  // (beyond `left` both are zero)
+      }
+      if (p.dz) st8<E>(p.dz, m * p.lddz + n, false, true, 8, d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += d[j];
+    }
+  }
+  if (!p.sums) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) lds[threadIdx.x * 9 + j] = sum[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < slab; i += 256) {
+    const int col = int(blockIdx.y) * slab + i;
+    if (col >= p.N) break;
+    float s = 0.f;
+    for (int k = 0; k < rows; ++k) s += lds[(k * p.lanes + (i >> 3)) * 9 + (i & 7)];
+    p.sums[int64_t(blockIdx.x) * p.N + col] = s;
+  }
+}
+
+// db[n] = sum of `parts` rows; 32 columns and 8 groups of rows per workgroup, the groups' sums added in order
+template <typename E>
+__global__ void __launch_bounds__(256) linear_colsum(const float* __restrict__ sums, int parts, int N,
+                                                     void* __restrict__ db, int f32) {
+  __shared__ float lds[8][32];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int n = int(blockIdx.x) * 32 + c;
+  float s = 0.f;
+  if (n < N) {
+#pragma unroll 8
+    for (int k = g; k < parts; k += 8) s += sums[int64_t(k) * N + n];
+  }
+  lds[g][c] = s;
+  __syncthreads();
+  if (g == 0 && n < N) {
+    for (int k = 1; k < 8; ++k) s += lds[k][c];
+    if (f32)
+      static_cast<float*>(db)[n] = s;
+    else
+      static_cast<uint16_t*>(db)[n] = E::down(s);
+  }
+}
+
+// ---- rows that are not 16-byte aligned, copied with their ends filled with zeros ------
+__global__ void __launch_bounds__(256) linear_pack(const uint16_t* __restrict__ src, int64_t ld, int rows, int cols,
+                                                   uint16_t* __restrict__ dst, int per_row) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= int64_t(rows) * per_row) return;
+  const int64_t r = i / per_row;
+  const int c = int(i - r * per_row) * 8;
+  union {
+    uint4 u;
+    uint16_t h[8];
+  } w;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w.h[j] = c + j < cols ? src[r * ld + c + j] : uint16_t(0);
+  *reinterpret_cast<uint4*>(dst + i * 8) = w.u;
+}
+
+// ---------------------------------------------------------------------------- host
+int pad8(int n) { return (n + 7) / 8 * 8; }
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+bool packed(const void* p, int64_t ld, int cols) { return !(aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0); }
+int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Tiles and parts of one product.  128 x 128 where that alone makes three quarters of a workgroup per CU, or where
+// r is long enough to be split to it; else 64 x 64, which has four times the workgroups.  r is split while two
+// workgroups per CU are not reached and each part keeps 256 values of r.
+struct Plan {
+  int tile, splits, r_per_split;
+  size_t bytes;
+};
+Plan plan_of(int M, int N, int r) {
+  Plan p;
+  const int64_t big = div_up(M, 128) * div_up(N, 128), small = div_up(M, 64) * div_up(N, 64);
+  p.tile = big >= 192 || (M > 64 && N > 64 && big * (r / 512) >= 192) ? 128 : 64;
+  const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64 or 128)
+  if (forced == 64 || forced == 128) p.tile = forced;
+  const int64_t tiles = p.tile == 128 ? big : small;
+  int64_t s = tiles >= 192 ? 1 : 512 / tiles;
+  const int64_t most = r / 256;
+  s = s > most ? most : s;
+  s = s < 1 ? 1 : s;
+  p.r_per_split = int(div_up(div_up(r, s), kR) * kR);
+  p.splits = int(div_up(r, p.r_per_split));
+  p.bytes = p.splits > 1 ? align256(size_t(p.splits) * M * N * sizeof(float)) : 0;
+  return p;
+}
+
+template <typename E, bool AC, bool BC>
+gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
+  g.splits = plan.splits;
+  g.r_per_split = plan.r_per_split;
+  g.part = static_cast<float*>(part);
+  const int64_t tm = div_up(g.M, plan.tile);
+  g.tiles_n = int(div_up(g.N, plan.tile));
+  const int64_t grid = tm * g.tiles_n * plan.splits;
+  GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
+  if (plan.tile == 128)
+    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+  else
+    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 2, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+  GD_LAUNCH_CHECK("linear_gemm");
+  if (plan.splits > 1) {
+    const int64_t blocks = div_up(int64_t(g.M) * ((g.N + 7) / 8), 256);
+    GD_REQUIRE(blocks < (int64_t(1) << 31), "linear: grid too large");
+    hipLaunchKernelGGL(linear_finish<E>, dim3(unsigned(blocks)), dim3(256), 0, s, g.part, plan.splits, g.M, g.N, g.epi);
+    GD_LAUNCH_CHECK("linear_finish");
+  }
+  return GD_OK;
+}
+
+// an operand's rows: as they are, or packed into the workspace
+struct Rows {
+  const uint16_t* p;
+  int64_t ld;
+  int cols;  // readable, a multiple of 8
+};
+gd_status rows_of(const void* p, int64_t ld, int rows, int cols, char** ws, Rows* out, hipStream_t s) {
+  if (!packed(p, ld, cols)) {
+    *out = {static_cast<const uint16_t*>(p), ld, cols};
+    return GD_OK;
+  }
+  const int per_row = pad8(cols) / 8;
+  const int64_t blocks = div_up(int64_t(rows) * per_row, 256);
+  GD_REQUIRE(blocks < (int64_t(1) << 31), "linear: grid too large");
+  uint16_t* dst = reinterpret_cast<uint16_t*>(*ws);
+  *ws += align256(size_t(rows) * per_row * 16);
+  if (rows > 0) {
+    hipLaunchKernelGGL(linear_pack, dim3(unsigned(blocks)), dim3(256), 0, s, static_cast<const uint16_t*>(p), ld, rows,
+                       cols, dst, per_row);
+    GD_LAUNCH_CHECK("linear_pack");
+  }
+  *out = {dst, pad8(cols), pad8(cols)};
+  return GD_OK;
+}
+size_t rows_bytes(bool pack, int rows, int cols) { return pack ? align256(size_t(rows) * pad8(cols) * 2) : 0; }
+
+Epi plain_epi(void* y, bool f32, int64_t ldy) {
+  Epi e = {};
+  e.y = y;
+  e.y_f32 = f32;
+  e.ldy = ldy;
+  e.y_vec = aligned(y, 16) && ldy % (f32 ? 4 : 8) == 0;
+  return e;
+}
+
+// workgroups along the rows of linear_dact: about 1024 in all, each of at least 32 rows per lane group
+struct DactPlan {
+  int lanes, slabs, blocks;
+  int64_t rows;
+};
+DactPlan dact_plan(int M, int N) {
+  DactPlan d;
+  d.lanes = 64;
+  while (d.lanes > 1 && d.lanes / 2 * 8 >= N) d.lanes /= 2;
+  d.slabs = int(div_up(N, 8 * d.lanes));
+  const int64_t group = 256 / d.lanes;
+  int64_t rows = div_up(M, div_up(1024, d.slabs));
+  rows = div_up(rows < 4 * group ? 4 * group : rows, group) * group;
+  d.rows = rows;
+  d.blocks = int(div_up(M, rows));
+  return d;
+}
+
+#define GD_TRY(expr)                     \
+  do {                                   \
+    const gd_status _s = (expr);         \
+    if (_s != GD_OK) return _s;          \
+  } while (0)
+
+gd_status check_shape(int dtype, int act, int M, int K, int N) {
+  GD_REQUIRE(dtype == GD_BF16 || dtype == GD_F16, "linear: bf16 or fp16 operands");
+  GD_REQUIRE(act >= kNone && act <= kSilu, "linear: activation %d", act);
+  GD_REQUIRE(M >= 0 && K > 0 && N > 0, "linear: M=%d K=%d N=%d", M, K, N);
+  // (tile origins and chunk ends stay in int, padded extents too)
+  GD_REQUIRE(M <= (1 << 30) && K <= (1 << 30) && N <= (1 << 30), "linear: M=%d K=%d N=%d", M, K, N);
+  return GD_OK;
+}
+
+template <typename E>
+gd_status forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int act, const void* res,
+                  int res_dtype, int64_t ldr, int M, int K, int N, void* y, int y_dtype, int64_t ldy, void* z,
+                  int64_t ldz, char* ws, hipStream_t s) {
+  Rows rx, rw;
+  GD_TRY(rows_of(x, ldx, M, K, &ws, &rx, s));
+  GD_TRY(rows_of(w, ldw, N, K, &ws, &rw, s));
+  Gemm g = {};
+  g.a = rx.p;
+  g.lda = rx.ld;
+  g.b = rw.p;
+  g.ldb = rw.ld;
+  g.M = M;
+  g.N = N;
+  g.ra = rx.cols;
+  g.rb = rw.cols;
+  g.epi = plain_epi(y, y_dtype == GD_F32, ldy);
+  g.epi.bias = static_cast<const uint16_t*>(bias);
+  g.epi.bias_vec = aligned(bias, 16);
+  g.epi.act = act;
+  g.epi.res = res;
+  g.epi.res_f32 = res_dtype == GD_F32;
+  g.epi.ldr = ldr;
+  g.epi.res_vec = aligned(res, 16) && ldr % (g.epi.res_f32 ? 4 : 8) == 0;
+  g.epi.z = static_cast<uint16_t*>(z);
+  g.epi.ldz = ldz;
+  return product<E, false, false>(plan_of(M, N, rx.cols), g, ws, s);
+}
+
+template <typename E>
+gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const void* z, int64_t ldz, const void* x,
+                   int64_t ldx, const void* w, int64_t ldw, int M, int K, int N, void* dx, int dx_dtype,
+                   int64_t lddx, void* dw, void* db, int param_dtype, char* ws, hipStream_t s) {
+  const int n8 = pad8(N);
+  Rows rz = {static_cast<const uint16_t*>(dy), lddy, N};
+  const bool make = act != kNone || dy_dtype == GD_F32 || packed(dy, lddy, N);
+  if (make && (dx || dw)) {
+    rz = {reinterpret_cast<uint16_t*>(ws), n8, n8};
+    ws += align256(size_t(M) * n8 * 2);
+  }
+  if (db || (make && (dx || dw))) {
+    const DactPlan d = dact_plan(M, N);
+    Dact a = {};
+    a.dy = dy;
+    a.lddy = lddy;
+    a.dy_f32 = dy_dtype == GD_F32;
+    a.dy_vec = aligned(dy, 16) && lddy % (a.dy_f32 ? 4 : 8) == 0;
+    a.z = act == kNone ? nullptr : static_cast<const uint16_t*>(z);
+    a.ldz = ldz;
+    a.z_vec = aligned(z, 16) && ldz % 8 == 0;
+    a.act = act;
+    a.dz = make && (dx || dw) ? const_cast<uint16_t*>(rz.p) : nullptr;
+    a.lddz = n8;
+    a.M = M;
+    a.N = N;
+    a.rows = d.rows;
+    a.lanes = d.lanes;
+    if (db) {
+      a.sums = reinterpret_cast<float*>(ws);
+      ws += align256(size_t(d.blocks) * N * sizeof(float));
+    }
+    hipLaunchKernelGGL(linear_dact<E>, dim3(d.blocks, d.slabs), dim3(256), 0, s, a);
+    GD_LAUNCH_CHECK("linear_dact");
+    if (db) {
+      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(256), 0, s, a.sums, d.blocks, N,
+                         db, int(param_dtype == GD_F32));
+      GD_LAUNCH_CHECK("linear_colsum");
+    }
+  }
+  if (dx) {
+    Rows rw;
+    GD_TRY(rows_of(w, ldw, N, K, &ws, &rw, s));
+    Gemm g = {};
+    g.a = rz.p;
+    g.lda = rz.ld;
+    g.ra = rz.cols;
+    g.b = rw.p;
+    g.ldb = rw.ld;
+    g.rb = N;
+    g.cb = rw.cols;
+    g.M = M;
+    g.N = K;
+    g.epi = plain_epi(dx, dx_dtype == GD_F32, lddx);
+    const Plan p = plan_of(M, K, n8);
+    GD_TRY((product<E, false, true>(p, g, ws, s)));
+    ws += p.bytes;
+  }
+  if (dw) {
+    Rows rx;
+    GD_TRY(rows_of(x, ldx, M, K, &ws, &rx, s));
+    Gemm g = {};
+    g.a = rz.p;
+    g.lda = rz.ld;
+    g.ca = rz.cols;
+    g.b = rx.p;
+    g.ldb = rx.ld;
+    g.cb = rx.cols;
+    g.ra = g.rb = M;
+    g.M = N;
+    g.N = K;
+    g.epi = plain_epi(dw, param_dtype == GD_F32, K);
+    GD_TRY((product<E, true, true>(plan_of(N, K, M), g, ws, s)));
+  }
+  return GD_OK;
+}
+
+size_t forward_bytes(bool pack_x, bool pack_w, int M, int K, int N) {
+  return rows_bytes(pack_x, M, K) + rows_bytes(pack_w, N, K) + plan_of(M, N, pad8(K)).bytes;
+}
+
+size_t backward_bytes(int M, int K, int N, bool dx, bool dw, bool db, bool pack_x, bool pack_w) {
+  const int n8 = pad8(N);
+  size_t b = dx || dw ? align256(size_t(M) * n8 * 2) : 0;
+  if (db) b += align256(size_t(dact_plan(M, N).blocks) * N * sizeof(float));
+  if (dx) b += rows_bytes(pack_w, N, K) + plan_of(M, K, n8).bytes;
+  if (dw) b += rows_bytes(pack_x, M, K) + plan_of(N, K, M).bytes;
+  return b;
+}
+
+}  // namespace
+}  // namespace gd
+
+using namespace gd;
+
+extern "C" size_t gd_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
+                                                    int K, int N) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  return forward_bytes(packed(x, ldx, K), packed(w, ldw, K), M, K, N);
+}
+
+extern "C" gd_status gd_linear_forward(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                       const void* bias, int act, const void* residual, int residual_dtype,
+                                       int64_t ldr, int M, int K, int N, void* y, int y_dtype, int64_t ldy, void* z,
+                                       int64_t ldz, void* workspace, size_t workspace_bytes, gd_stream_t stream) {
+  GD_TRY(check_shape(dtype, act, M, K, N));
+  if (M == 0) return GD_OK;
+  GD_REQUIRE(x && w && y && ldx >= K && ldw >= K && ldy >= N, "linear: null pointer or short rows");
+  GD_REQUIRE(aligned(x, 2) && aligned(w, 2) && aligned(bias, 2), "linear: misaligned operands");
+  GD_REQUIRE(!residual || (ldr >= N && (residual_dtype == dtype || residual_dtype == GD_F32)),
+             "linear: the residual is fp32 or of the operands' type");
+  GD_REQUIRE(y_dtype == (residual ? residual_dtype : dtype), "linear: y has the residual's type, without one x's");
+  GD_REQUIRE(aligned(y, y_dtype == GD_F32 ? 4 : 2) && aligned(residual, residual_dtype == GD_F32 ? 4 : 2),
+             "linear: misaligned y or residual");
+  GD_REQUIRE(!z || (aligned(z, 16) && ldz % 8 == 0 && ldz >= pad8(N)), "linear: z has rows padded to 8 values");
+  const size_t want = forward_bytes(packed(x, ldx, K), packed(w, ldw, K), M, K, N);
+  GD_REQUIRE(workspace_bytes >= want && (want == 0 || (workspace && aligned(workspace, 16))),
+             "linear: workspace of %zu bytes, %zu wanted", workspace_bytes, want);
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t s = as_hip(stream);
+  return dtype == GD_BF16 ? forward<Bf16>(x, ldx, w, ldw, bias, act, residual, residual_dtype, ldr, M, K, N, y, y_dtype,
+                                          ldy, z, ldz, ws, s)
+                          : forward<Fp16>(x, ldx, w, ldw, bias, act, residual, residual_dtype, ldr, M, K, N, y, y_dtype,
+                                          ldy, z, ldz, ws, s);
+}
+
+extern "C" size_t gd_linear_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
+                                                     int K, int N, int dx, int dw, int db) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  return backward_bytes(M, K, N, dx, dw, db, packed(x, ldx, K), packed(w, ldw, K));
+}
+
+extern "C" gd_status gd_linear_backward(int dtype, int act, const void* dy, int dy_dtype, int64_t lddy, const void* z,
+                                        int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
+                                        int K, int N, void* dx, int dx_dtype, int64_t lddx, void* dw, void* db,
+                                        int param_dtype, void* workspace, size_t workspace_bytes,
+                                        gd_stream_t stream) {
+  GD_TRY(check_shape(dtype, act, M, K, N));
+  GD_REQUIRE(M > 0, "linear: gradients of no rows");
+  GD_REQUIRE(dy && x && w && lddy >= N && ldx >= K && ldw >= K && (!dx || lddx >= K), "linear: null pointer or short rows");
+  GD_REQUIRE(dy_dtype == dtype || dy_dtype == GD_F32, "linear: dy is fp32 or of the operands' type");
+  GD_REQUIRE((dx_dtype == dtype || dx_dtype == GD_F32) && (param_dtype == dtype || param_dtype == GD_F32),
+             "linear: gradients are fp32 or of the operands' type");
+  GD_REQUIRE(act == kNone || (z && ldz >= N), "linear: the activation's slope needs z");
+  GD_REQUIRE(aligned(dy, dy_dtype == GD_F32 ? 4 : 2) && aligned(z, 2) && aligned(x, 2) && aligned(w, 2) &&
+                 aligned(dx, dx_dtype == GD_F32 ? 4 : 2) && aligned(dw, param_dtype == GD_F32 ? 4 : 2) &&
+                 aligned(db, param_dtype == GD_F32 ? 4 : 2),
+             "linear: misaligned operands");
+  const size_t want = backward_bytes(M, K, N, dx, dw, db, packed(x, ldx, K), packed(w, ldw, K));
+  GD_REQUIRE(workspace_bytes >= want && (want == 0 || (workspace && aligned(workspace, 16))),
+             "linear: workspace of %zu bytes, %zu wanted", workspace_bytes, want);
+  GD_REQUIRE(dact_plan(M, N).slabs < 65536, "linear: N=%d", N);
+  char* ws = static_cast<char*>(workspace);
+  hipStream_t s = as_hip(stream);
+  return dtype == GD_BF16 ? backward<Bf16>(act, dy, dy_dtype, lddy, z, ldz, x, ldx, w, ldw, M, K, N, dx, dx_dtype, lddx,
+                                           dw, db, param_dtype, ws, s)
+                          : backward<Fp16>(act, dy, dy_dtype, lddy, z, ldz, x, ldx, w, ldw, M, K, N, dx, dx_dtype, lddx,
+                                           dw, db, param_dtype, ws, s);
+}

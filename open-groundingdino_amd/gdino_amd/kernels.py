@@ -15,6 +15,8 @@ primitives, so that the implementation behind each op is one swap:
   contrastive_logits ContrastiveEmbed            utils.py:242-273
   contrastive_rowmax its max over tokens, the two-stage proposal score
                      (transformer.py:292-296), without the [B, S, 256] logits
+  linear_act         activation(x W^T + b) + residual, the feed-forward layers
+                     (transformer.py:784-808): gdino_amd/linear.py
 
 ``IMPL[name]`` selects the implementation; ``"hip"`` entries are the
 hand-written gfx950 kernels of csrc/ (registered by their modules when the
@@ -155,6 +157,11 @@ def contrastive_rowmax(x, text, text_token_mask):
     return get("contrastive_rowmax")(x, text, text_token_mask)
 
 
+def linear_act(x, weight, bias=None, activation="none", residual=None):
+    """activation(x @ weight.T + bias) + residual (gdino_amd/linear.py)."""
+    return get("linear_act")(x, weight, bias, activation, residual)
+
+
 # HIP implementations register themselves as the defaults for CUDA tensors.
 from . import biattn  # noqa: E402,F401
 from . import wattn  # noqa: E402,F401
@@ -164,3 +171,4 @@ from . import msda_prologue  # noqa: E402,F401
 from . import wgrad  # noqa: E402,F401
 from . import layernorm  # noqa: E402,F401
 from . import lsap  # noqa: E402,F401  (the device Hungarian matching)
+from . import linear  # noqa: E402,F401

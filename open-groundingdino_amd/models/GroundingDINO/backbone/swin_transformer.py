@@ -22,7 +22,7 @@ import torch.nn.functional as F
 import torch.utils.checkpoint as checkpoint
 
 from gdino_amd.conv import GemmConv2d
-from gdino_amd import castcache, kernels
+from gdino_amd import castcache, kernels, linear
 from gdino_amd.layernorm import add_scaled_norm, layer_norm
 from gdino_amd.misc import DropPath, NestedTensor, add_drop_path, to_2tuple, trunc_normal_
 
@@ -38,6 +38,9 @@ class Mlp(nn.Module):
         self.drop = nn.Dropout(drop)
 
     def forward(self, x):
+        if linear.FUSED_MLP and type(self.act) is nn.GELU and linear.supported(x, self.fc1.weight):
+            return self.drop(linear.mlp(x, self.fc1, self.fc2, "gelu" if self.act.approximate == "none" else "gelu_tanh",
+                                        self.drop))
         return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))
 
 

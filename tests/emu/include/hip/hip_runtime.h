@@ -388,6 +388,24 @@ inline C4 mfma_16x16x32_bf16(V8 a, V8 b, C4 c) {
   return d;
 }
 
+// v_mfma_f32_16x16x32_f16: the same lane maps
+template <typename V8, typename C4>
+inline C4 mfma_16x16x32_f16(V8 a, V8 b, C4 c) {
+  static_assert(sizeof(V8) == 16 && sizeof(C4) == 16, "f16x8 / f32x4 operands");
+  struct Ops { V8 a, b; } mine{a, b}, all[64];
+  wave_gather(&mine, sizeof(Ops), all);
+  const unsigned l = lane_id();
+  C4 d;
+  for (int r = 0; r < 4; ++r) {
+    const int row = 4 * int(l >> 4) + r, col = int(l & 15);
+    double acc = 0.0;
+    for (int k = 0; k < 32; ++k)
+      acc += double(float(all[row + 16 * (k >> 3)].a[k & 7])) * double(float(all[col + 16 * (k >> 3)].b[k & 7]));
+    d[r] = float(double(c[r]) + acc);
+  }
+  return d;
+}
+
 // v_mfma_f32_16x16x4_f32: lane l holds A[l&15][l>>4] and B[l>>4][l&15].
 template <typename C4>
 inline C4 mfma_16x16x4_f32(float a, float b, C4 c) {
@@ -456,6 +474,8 @@ inline int __ffsll(long long v) { return __builtin_ffsll(v); }
   ::gd_emu::mfma_16x16x32_bf16((a), (b), (c))
 #define __builtin_amdgcn_cvt_pk_f32_fp8(w, hi) ::gd_emu::cvt_pk_f32_fp8((w), (hi))
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, hi) ::gd_emu::cvt_pk_fp8_f32((a), (b), (old), (hi))
+#define __builtin_amdgcn_rcpf(x) (1.0f / (x))
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, cbsz, abid, blgp) ::gd_emu::mfma_16x16x32_f16((a), (b), (c))
 #define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) ::gd_emu::fdot2_bf16((a), (b), (c))
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) ::gd_emu::mfma_16x16x4_f32((a), (b), (c))
 #define hipLaunchKernelGGL(kernel, g, b, shm, stream, ...) \

@@ -1,0 +1,101 @@
+"""The linear layer and its gradients in 64 bits, with bounds of the kernels' roundings (shared by the emulator and
+the GPU tests)."""
+import math
+
+import torch
+
+U = 2.0 ** -24  # half a step of fp32
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def act64(z, name):
+    if name == "none":
+        return z.clone()
+    if name == "relu":
+        return torch.relu(z)
+    if name == "gelu":
+        return z * torch.special.ndtr(z)
+    if name == "gelu_tanh":
+        return 0.5 * z * (1 + torch.tanh(math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3)))
+    return z * torch.sigmoid(z)
+
+
+def inputs(m, k, n, dtype, bias=True, residual=None, seed=0, device="cpu", grad=True):
+    g = torch.Generator().manual_seed(seed)
+
+    def leaf(t, dt):
+        return t.to(dt).to(device).requires_grad_(grad)
+
+    x, w = leaf(torch.randn(m, k, generator=g), dtype), leaf(torch.randn(n, k, generator=g) * k ** -0.5, dtype)
+    b = leaf(torch.randn(n, generator=g) * 0.3, dtype) if bias else None
+    r = leaf(torch.randn(m, n, generator=g), residual) if residual is not None else None
+    dy = torch.randn(m, n, generator=g).to(residual or dtype).to(device)
+    return x, w, b, r, dy
+
+
+def check(x, w, b, act, r, y, dy=None, grads=None, low=None):
+    """y (and grads = (dx, dw, db, dr), None where not given) against 64 bits.  ``low``: the type the kernels read x
+    and w in, where they are cast.  The bounds, term by term:
+      z      K + 2 additions in fp32 of exact products
+      act    Lipschitz below 1.13; its own evaluation to 2e-6 of (1 + |z|)
+      y      one rounding to its type
+      dz     act'(z) from z rounded (|z act''| < 0.5) and off by z's error (|act''| < 1.1; a ReLU's z may change its
+             sign there); then dz is rounded
+      dx, dw, db   those errors through the product, its fp32 additions (db: unrounded dz), one rounding"""
+    dt = low or x.dtype
+    u = half_step(dt)
+    x64, w64 = (t.detach().cpu().to(dt).double() for t in (x, w))
+    m, k = x64.shape
+    n = w64.shape[0]
+    z = x64 @ w64.t()
+    size = x64.abs() @ w64.abs().t()
+    if b is not None:
+        b64 = b.detach().cpu().to(dt).double()
+        z, size = z + b64, size + b64.abs()
+    ez = (k + 2) * U * size
+    want = act64(z, act)
+    ey = 1.13 * ez + (2e-6 * (1 + z.abs()) if act not in ("none", "relu") else 0)
+    if r is not None:
+        want = want + r.detach().cpu().double()
+        ey = ey + U * want.abs()
+    tiny = 2.0 ** -25 if y.dtype == torch.float16 else 1e-38
+    near(y, want, ey + tiny)
+    if dy is None:
+        return
+    d = dy.cpu().double()
+    zz = z.clone().requires_grad_()
+    s = torch.autograd.grad(act64(zz, act).sum(), zz)[0]
+    dz = d * s
+    raw = torch.zeros_like(dz) if act == "none" else d.abs() * (1.1 * ez + 2e-6)
+    if act == "relu":
+        raw = torch.where(z.abs() <= ez, d.abs(), torch.zeros_like(d))
+    elif act != "none":
+        raw = raw + 0.5 * u * d.abs()
+    e = raw + (0 if act == "none" and dy.dtype == dt else u * (dz.abs() + raw) + tiny)
+    dx, dw, db, dr = grads
+    if dx is not None:
+        near(dx, dz @ w64, e @ w64.abs() + (n + 2) * U * (dz.abs() @ w64.abs()) + tiny)
+    if dw is not None:
+        near(dw, dz.t() @ x64, e.t() @ x64.abs() + (m + 2) * U * (dz.abs().t() @ x64.abs()) + tiny)
+    if db is not None:
+        near(db, dz.sum(0), raw.sum(0) + (m + 2) * U * dz.abs().sum(0) + tiny)
+    if dr is not None:
+        assert torch.equal(dr.cpu(), dy.to(dr.dtype).cpu())
+
+
+def near(got, want, bound):
+    """Within the bound and one rounding to got's type."""
+    off = (got.detach().cpu().double() - want).abs()
+    assert torch.isfinite(got).all() and (off <= bound + half_step(got.dtype) * (want.abs() + bound)).all(), \
+        float((off / (bound + half_step(got.dtype) * (want.abs() + bound))).max())
+
+
+def run(x, w, b, act, r, dy):
+    from gdino_amd.linear import linear_act
+    y = linear_act(x, w, b, act, r)
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    got = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, dy)))
+    return y, tuple(None if t is None else got[id(t)] for t in (x, w, b, r))

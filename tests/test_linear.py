@@ -1,0 +1,202 @@
+"""gdino_amd.linear without a GPU: the kernels' sources in the emulator (tests/emu), refusals, and the wiring."""
+import pytest
+import torch
+
+import emu_product
+import linear_cases as lc
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture
+def emulated():
+    with emu_product.emulated_product():
+        yield
+
+
+# 64-tiles with ragged edges, rows that have to be packed, one row, 128-tiles, a split sum
+@pytest.mark.parametrize("m,k,n,act,dtype,residual,bias", [
+    (1, 8, 8, "none", BF, None, True),
+    (5, 24, 72, "relu", BF, None, True),
+    (70, 40, 65, "gelu", BF, BF, True),
+    (33, 17, 9, "silu", HF, HF, True),
+    (66, 130, 30, "gelu_tanh", HF, F32, False),
+    (3, 600, 16, "none", BF, F32, True),
+    (2, 1, 1, "relu", BF, BF, False),
+])
+def test_linear_act(emulated, m, k, n, act, dtype, residual, bias):
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, bias, residual, seed=m)
+    y, grads = lc.run(x, w, b, act, r, dy)
+    assert y.dtype == (residual or dtype)
+    lc.check(x, w, b, act, r, y, dy, grads)
+
+
+@pytest.mark.parametrize("tile", ["64", "128"])
+@pytest.mark.parametrize("m,k,n,act,dtype", [(150, 72, 136, "gelu", BF), (129, 200, 8, "none", HF),
+                                             (1100, 8, 24, "relu", BF), (3, 1030, 16, "silu", BF)])
+def test_tiles(emulated, monkeypatch, tile, m, k, n, act, dtype):
+    """Both tiles in every layout of the operands, with ragged edges and with sums over r that are split."""
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, True, None, seed=2)
+    y, grads = lc.run(x, w, b, act, r, dy)
+    lc.check(x, w, b, act, r, y, dy, grads)
+
+
+def test_strides_and_shapes(emulated):
+    """Leading dimensions, transposed and sliced inputs, an expanded residual and gradient, a misaligned view."""
+    from gdino_amd.linear import linear_act
+    x, w, b, _, _ = lc.inputs(24, 48, 40, BF, seed=4, grad=False)
+    base = torch.randn(4, 6, 48).to(BF)
+    cases = [base, base.transpose(0, 1), base[:, :, ::1][1:], torch.randn(6, 4, 96).to(BF)[..., :48],
+             torch.randn(24 * 48 + 1).to(BF)[1:].view(4, 6, 48)]
+    for t in cases:
+        y = linear_act(t, w, b, "relu")
+        assert y.shape == t.shape[:-1] + (40,)
+        lc.check(t.reshape(-1, 48), w, b, "relu", None, y.reshape(-1, 40))
+    y = linear_act(base, w.t().contiguous().t(), b, "none")  # a weight with its output features contiguous
+    lc.check(base.reshape(-1, 48), w, b, "none", None, y.reshape(-1, 40))
+    xs = base.clone().requires_grad_()
+    rs = torch.randn(40).to(BF).requires_grad_()
+    linear_act(xs, w, b, "none", rs.expand(4, 6, 40)).sum().backward()
+    assert torch.equal(rs.grad, torch.full((40,), 24.0, dtype=BF))
+    one = torch.ones(24, 40, dtype=BF)
+    lc.near(xs.grad.reshape(-1, 48), one.double() @ w.double(), 42 * lc.U * (one.double() @ w.double().abs()))
+    assert linear_act(x[0], w, b).shape == (40,)
+
+
+def test_partial_gradients(emulated):
+    """Only what is asked for, and nothing saved or written for what is not."""
+    from gdino_amd.linear import linear_act
+    for which in range(4):
+        x, w, b, r, dy = lc.inputs(9, 24, 16, BF, True, BF, seed=5, grad=False)
+        leaf = (x, w, b, r)[which].requires_grad_()
+        y = linear_act(x, w, b, "gelu", r)
+        g = torch.autograd.grad(y, leaf, dy)[0]
+        grads = [None] * 4
+        grads[which] = g
+        lc.check(x, w, b, "gelu", r, y, dy, grads)
+    with torch.no_grad():
+        assert not linear_act(x, w, b.requires_grad_(), "gelu", r).requires_grad
+
+
+def test_rows_of_nothing(emulated):
+    from gdino_amd.linear import linear_act
+    x, w, b, r, dy = lc.inputs(0, 24, 16, BF, True, F32)
+    y = linear_act(x, w, b, "relu", r)
+    assert y.shape == (0, 16) and y.dtype == F32
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert dx.shape == (0, 24) and not dw.any() and not db.any()
+
+
+def test_autocast_and_masters(emulated):
+    """fp32 leaves under bf16 autocast: the product in bf16, gradients in fp32."""
+    from gdino_amd import castcache
+    from gdino_amd.linear import linear_act, mlp
+    castcache.clear()
+    x, w, b, r, dy = lc.inputs(20, 24, 16, F32, True, F32, seed=6)
+    with torch.autocast("cpu", dtype=BF):
+        y, grads = lc.run(x, w, b, "gelu", r, dy)
+    assert y.dtype == F32 and all(g.dtype == F32 for g in grads)
+    lc.check(x, w, b, "gelu", r, y, dy, grads, low=BF)
+    fc1, fc2 = torch.nn.Linear(24, 40), torch.nn.Linear(40, 24)
+    with torch.autocast("cpu", dtype=BF):
+        out = mlp(x, fc1, fc2, "gelu", torch.nn.Dropout(0.0))
+        ref = fc2(torch.nn.functional.gelu(fc1(x)))
+    assert out.dtype == BF
+    # both round h and the result to bf16; the composition also rounds before the GELU: two roundings of h, |w| summed
+    size = (fc1(x).abs() + 1) @ fc2.weight.abs().t() + fc2.bias.abs()
+    assert ((out - ref).abs() <= 4 * lc.half_step(BF) * size).all()
+    out.float().sum().backward()
+    assert fc1.weight.grad.dtype == F32 and fc1.weight.grad.abs().sum() > 0
+
+
+def test_differences(emulated):
+    """The gradient of x against differences of the forward in 64 bits, and the wiring against each leaf."""
+    x, w, b, r, dy = lc.inputs(4, 16, 8, HF, True, HF, seed=7)
+    y, (dx, dw, db, dr) = lc.run(x, w, b, "silu", r, dy)
+
+    def loss(x, w, b):
+        return float((lc.act64(x @ w.t() + b, "silu") * dy.double()).sum())
+
+    args = [t.detach().double() for t in (x, w, b)]
+    h = 1e-5
+    for i, g in enumerate((dx, dw, db)):
+        step = torch.randn(args[i].shape, generator=torch.Generator().manual_seed(i)).double()
+        up, down = ([a + s * h * step if j == i else a for j, a in enumerate(args)] for s in (1, -1))
+        want = (loss(*up) - loss(*down)) / (2 * h)
+        # each gradient value carries a rounding of itself and of the dz it sums: 3 half steps of its size, and more
+        # where terms cancel; the direction's sum is held to 8 of the sizes
+        assert abs(float((g.double() * step).sum()) - want) <= 8 * lc.half_step(HF) * float((g.double() * step).abs().sum())
+
+
+def test_refusals(emulated):
+    from gdino_amd import _lib
+    from gdino_amd.linear import linear_act
+    x, w, b, r, _ = lc.inputs(6, 24, 16, BF, True, BF, grad=False)
+    with pytest.raises(ValueError, match="activation"):
+        linear_act(x, w, b, "swish")
+    with pytest.raises(ValueError, match="do not match"):
+        linear_act(x[:, :8], w, b)
+    with pytest.raises(ValueError, match="do not match"):
+        linear_act(x[:, :0], w[:, :0], b)
+    with pytest.raises(ValueError, match="bias"):
+        linear_act(x, w, b[:8])
+    with pytest.raises(ValueError, match="residual"):
+        linear_act(x, w, b, "none", r[:1])
+    with pytest.raises(TypeError, match="linear_act"):
+        linear_act(x.float(), w.float(), b.float())
+    with pytest.raises(TypeError, match="linear_act"):
+        linear_act(x, w.half(), b)
+    with pytest.raises(TypeError, match="linear_act"):
+        linear_act(x, w, b.float())
+    with pytest.raises(TypeError, match="residual"):
+        linear_act(x, w, b, "none", r.half())
+    y = torch.empty(6, 16, dtype=BF)
+    args = (2, x.data_ptr(), 24, w.data_ptr(), 24, None, 0, None, 2, 0, 6, 24, 16, y.data_ptr(), 2, 16, None, 0)
+    _lib.call("gd_linear_forward", *args, None, 0, None)
+    for bad in ({0: 0}, {2: 8}, {6: 9}, {11: 0}, {13: None}, {14: 0}, {16: y.data_ptr() + 2, 17: 16}):
+        call = [bad.get(i, a) for i, a in enumerate(args)]
+        with pytest.raises(_lib.GdError):
+            _lib.call("gd_linear_forward", *call, None, 0, None)
+    packed = [{2: 25}.get(i, a) for i, a in enumerate(args)]  # rows to pack, and no workspace
+    with pytest.raises(_lib.GdError, match="workspace"):
+        _lib.call("gd_linear_forward", *packed, None, 0, None)
+
+
+def test_cpu_tensors_raise():
+    from gdino_amd.linear import linear_act
+    x, w, b, _, _ = lc.inputs(6, 24, 16, BF, grad=False)
+    with pytest.raises(RuntimeError, match="Not implemented on the CPU"):
+        linear_act(x, w, b)
+
+
+def test_dispatch():
+    """kernels.linear_act composes library kernels where the layer does not apply (host tensors, fp32)."""
+    from gdino_amd import kernels
+    x, w, b, r, _ = lc.inputs(6, 24, 16, F32, True, F32, grad=False)
+    for act in ("none", "relu", "gelu", "gelu_tanh", "silu"):
+        y = kernels.linear_act(x, w, b, act, r)
+        want = lc.act64(x.double() @ w.double().t() + b.double(), act) + r.double()
+        torch.testing.assert_close(y.double(), want, rtol=1e-5, atol=1e-5)
+
+
+def test_swin_mlp_runs_on_it(emulated, monkeypatch):
+    """GDINO_FUSED_MLP: the backbone's MLP, off by default, calls the layer under autocast and keeps its result."""
+    from gdino_amd import castcache, linear
+    from models.GroundingDINO.backbone.swin_transformer import Mlp
+    castcache.clear()
+    assert not linear.FUSED_MLP
+    torch.manual_seed(0)
+    net, x = Mlp(24, 40), torch.randn(5, 7, 24)
+    calls = []
+    inner = linear.linear_act
+    monkeypatch.setattr(linear, "linear_act", lambda *a, **k: calls.append(1) or inner(*a, **k))
+    with torch.autocast("cpu", dtype=BF):
+        want = net(x)
+        assert not calls
+        monkeypatch.setattr(linear, "FUSED_MLP", True)
+        got = net(x)
+    assert len(calls) == 2 and got.dtype == want.dtype
+    size = (net.fc1(x).abs() + 1) @ net.fc2.weight.abs().t() + net.fc2.bias.abs()
+    assert ((got - want).abs() <= 4 * lc.half_step(BF) * size).all()
+    assert net(x.double().float()).dtype == F32  # without autocast: the plain composition

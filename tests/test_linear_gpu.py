@@ -1,0 +1,160 @@
+"""gdino_amd.linear on the device, against 64 bits: sizes, strides, types, capture, streams."""
+import pytest
+import torch
+
+import linear_cases as lc
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.mark.parametrize("m,k,n,act,dtype,residual,bias", [
+    (1, 256, 256, "none", BF, F32, True),
+    (1, 1, 1, "gelu", BF, None, True),
+    (7, 1000, 3, "silu", HF, HF, False),
+    (64, 64, 64, "relu", HF, None, True),
+    (65, 1024, 4096, "gelu_tanh", BF, None, True),
+    (900, 256, 2048, "relu", BF, BF, True),
+    (1237, 331, 517, "silu", HF, HF, True),
+    (1801, 2048, 256, "none", BF, F32, True),
+    (2500, 257, 1030, "gelu", BF, None, False),
+    (8400, 96, 384, "gelu", BF, None, True),
+    (16, 4104, 72, "relu", BF, None, True),
+    (130, 8, 4096, "none", HF, None, True),
+])
+def test_linear_act(m, k, n, act, dtype, residual, bias):
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, bias, residual, seed=m, device="cuda")
+    y, grads = lc.run(x, w, b, act, r, dy)
+    assert y.dtype == (residual or dtype)
+    lc.check(x, w, b, act, r, y, dy, grads)
+
+
+@pytest.mark.parametrize("tile", ["64", "128"])
+@pytest.mark.parametrize("m,k,n", [(300, 136, 264), (257, 513, 127), (5, 2048, 520), (4100, 72, 40)])
+def test_tiles(monkeypatch, tile, m, k, n):
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    for dtype in (BF, HF):
+        x, w, b, r, dy = lc.inputs(m, k, n, dtype, True, F32, seed=k, device="cuda")
+        y, grads = lc.run(x, w, b, "gelu", r, dy)
+        lc.check(x, w, b, "gelu", r, y, dy, grads)
+
+
+def test_large_values():
+    """Activations far from zero: nothing overflows on the way to a finite result."""
+    from gdino_amd.linear import linear_act
+    x = torch.tensor([[30.0], [-30.0], [3000.0], [-3000.0], [0.0]], device="cuda")
+    w = torch.tensor([[1.0], [1e4]], device="cuda")
+    for act in ("relu", "gelu", "gelu_tanh", "silu"):
+        xs = x.bfloat16().requires_grad_()
+        ws = w.bfloat16()
+        y = linear_act(xs, ws, None, act)
+        z = xs.detach().double() @ ws.double().t()
+        torch.testing.assert_close(y.double(), torch.where(z > 0, z, torch.zeros_like(z)), rtol=2 ** -8, atol=1e-9)
+        y.sum().backward()
+        assert torch.isfinite(xs.grad).all()
+
+
+def test_nan_and_infinity_stay_in_their_rows():
+    from gdino_amd.linear import linear_act
+    x, w, b, _, dy = lc.inputs(300, 264, 136, BF, device="cuda", seed=3)
+    clean = linear_act(x, w, b, "gelu")
+    with torch.no_grad():
+        x[17, 5], x[250, 263] = float("nan"), float("inf")
+    y = linear_act(x, w, b, "gelu")
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    rows = torch.ones(300, dtype=torch.bool, device="cuda")
+    rows[[17, 250]] = False
+    assert torch.equal(y[rows], clean[rows]) and torch.isnan(y[17]).all() and torch.isfinite(dx[rows]).all()
+    assert torch.isnan(db).all()  # (the sum over rows holds the NaN)
+
+
+@pytest.mark.parametrize("shape", [(900, 256, 2048), (2, 4096, 40), (333, 129, 77)])
+def test_captured(shape):
+    """Forward and gradients in one graph, replayed on new values between eager work; bit by bit the eager result.
+    (torch.autograd.grad: the captured pass owns its whole graph, no accumulation node of an eager one takes part.)"""
+    from gdino_amd.linear import linear_act
+    m, k, n = shape
+    x, w, b, r, dy = lc.inputs(m, k, n, BF, True, F32, device="cuda")
+
+    def step(x, w, b, r):
+        y = linear_act(x, w, b, "gelu", r)
+        return (y.detach(),) + torch.autograd.grad(y, (x, w, b, r), dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(x, w, b, r)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = step(x, w, b, r)
+    for i in range(4):
+        with torch.no_grad():
+            for t in (x, w, b, r, dy):
+                t.mul_(0.75).add_(0.01 * i)
+        graph.replay()
+        want = step(x, w, b, r)
+        torch.cuda.synchronize()
+        for a, c in zip(out, want):
+            assert torch.equal(a, c), i
+
+
+def test_on_another_stream_and_two_at_once():
+    from gdino_amd.linear import linear_act
+    sets = [lc.inputs(1000 + i, 512, 384, BF, True, None, seed=i, device="cuda") for i in range(2)]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in sets], []
+    for s, (x, w, b, r, dy) in zip(streams, sets):
+        with torch.cuda.stream(s):
+            y = linear_act(x, w, b, "silu")
+            outs.append((y, torch.autograd.grad(y, (x, w, b), dy)))
+    torch.cuda.synchronize()
+    for (x, w, b, r, dy), (y, g) in zip(sets, outs):
+        lc.check(x, w, b, "silu", None, y, dy, g + (None,))
+
+
+def test_rows_behind_the_last_are_left():
+    """y, dx and dw end where their tensors end: what lies behind them in memory is untouched."""
+    from gdino_amd import _lib
+    m, k, n = 70, 72, 77
+    x, w, b, _, _ = lc.inputs(m, k, n, BF, device="cuda", grad=False)
+    y = torch.full((m * n + 4096,), 7.0, dtype=BF, device="cuda")
+    _lib.call("gd_linear_forward", 2, x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), 0, None, 2, 0, m, k, n,
+              y.data_ptr(), 2, n, None, 0, None, 0, _lib.stream_of(y))
+    assert (y[m * n:] == 7).all()
+    lc.check(x, w, b, "none", None, y[:m * n].view(m, n))
+
+
+def test_feed_forward_and_update_together():
+    """A two-layer block with a residual stream trained by the AdamW step, under autocast with fp32 weights, beside the
+    composition of library kernels: gradients agree to the two paths' roundings, weights to a few updates."""
+    from gdino_amd import castcache, optim
+    from gdino_amd.linear import linear_act
+    castcache.clear()
+    torch.manual_seed(0)
+    fc1, fc2 = torch.nn.Linear(192, 768).cuda(), torch.nn.Linear(768, 192).cuda()
+    ref1, ref2 = torch.nn.Linear(192, 768).cuda(), torch.nn.Linear(768, 192).cuda()
+    ref1.load_state_dict(fc1.state_dict())
+    ref2.load_state_dict(fc2.state_dict())
+    ours, theirs = [*fc1.parameters(), *fc2.parameters()], [*ref1.parameters(), *ref2.parameters()]
+    a = optim.AdamW(ours, lr=1e-3)
+    c = torch.optim.AdamW(theirs, lr=1e-3)
+    x = torch.randn(2048, 192, device="cuda")
+    for i in range(3):
+        with torch.autocast("cuda", dtype=BF):
+            y = linear_act(linear_act(x, fc1.weight, fc1.bias, "gelu"), fc2.weight, fc2.bias, "none", x)
+        z = x + ref2(torch.nn.functional.gelu(ref1(x)))
+        y.square().mean().backward()
+        z.square().mean().backward()
+        if i == 0:
+            for p, q in zip(ours, theirs):
+                assert p.grad.dtype == F32
+                # some five roundings to bf16 on the way of each term of the sums
+                assert float((p.grad - q.grad).norm()) <= 5 * lc.half_step(BF) * float(q.grad.norm())
+        a.step(max_norm=0.1)
+        torch.nn.utils.clip_grad_norm_(theirs, 0.1)
+        c.step()
+        a.zero_grad()
+        c.zero_grad()
+        for p, q in zip(ours, theirs):  # an update moves a weight by about lr, whichever way a tiny gradient rounds
+            assert float((p - q).detach().abs().max()) <= 2.5e-3 * (i + 1)
