@@ -299,6 +299,8 @@ def updated(s):
 
 # ------------------------------------------------------- the package's operators
 def package(name):
+    if "gdino_amd." + name in sys.modules:
+        return sys.modules["gdino_amd." + name]
     import importlib
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "open-groundingdino_amd")
     if at not in sys.path:
