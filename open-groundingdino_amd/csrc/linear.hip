@@ -202,15 +202,13 @@ struct Epi {
   bool bias_vec, res_f32, res_vec, y_f32, y_vec;
 };
 
+// 8 values of a row: bias b and residual r were loaded before (zeros where there is none)
 template <typename E>
-__device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N, float v[8]) {
+__device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N, const float b[8], const float r[8],
+                                          float v[8]) {
   const int left = N - n < 8 ? N - n : 8;
-  if (e.bias) {
-    float b[8];
-    ld8<E>(e.bias, n, false, e.bias_vec, left, b);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += b[j];
-  }
+  for (int j = 0; j < 8; ++j) v[j] += b[j];
   if (e.z) {
     float z[8];
 #pragma unroll
@@ -218,12 +216,8 @@ __device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N,
     st8<E>(e.z, m * e.ldz + n, false, true, 8, z);
   }
   activate8(v, e.act);
-  if (e.res) {
-    float r[8];
-    ld8<E>(e.res, m * e.ldr + n, e.res_f32, e.res_vec, left, r);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += r[j];
-  }
+  for (int j = 0; j < 8; ++j) v[j] += r[j];
   st8<E>(e.y, m * e.ldy + n, e.y_f32, e.y_vec, left, v);
 }
 
@@ -245,14 +239,16 @@ constexpr int kR = 64;  // values of r per staged chunk
 // Offset of 16-byte chunk ch of row r in an LDS image.  Rows image [x][64 r]: 128-byte rows; 16 lanes read the same
 // chunk of 16 consecutive rows, so the chunk index is xored with row / 2: with the row's parity that is every one of
 // the 16 positions of 256 bytes, all 64 banks.
-__device__ __forceinline__ int row_at(int row, int ch) { return row * kR + ((ch ^ ((row >> 1) & 7)) << 3); }
+__device__ __forceinline__ int row_swz(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int row_at(int row, int ch) { return row * kR + ((ch ^ row_swz(row)) << 3); }
 // Columns image [64 r][X]: the transposing read (ds_read_b64_tr_b16) of half a wave touches rows q and 8 + q, q < 4, 32
 // bytes each, which have to lie 32 bytes apart modulo 256.
 template <int X>
-__device__ __forceinline__ int col_at(int r, int ch) {
-  const int swz = X == 64 ? 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1) : 2 * (r & 3) + 8 * ((r >> 3) & 1);
-  return r * X + ((ch ^ swz) << 3);
+__device__ __forceinline__ int col_swz(int r) {
+  return X == 64 ? 2 * ((r >> 1) & 1) + 4 * ((r >> 3) & 1) : 2 * (r & 3) + 8 * ((r >> 3) & 1);
 }
+template <int X>
+__device__ __forceinline__ int col_at(int r, int ch) { return r * X + ((ch ^ col_swz<X>(r)) << 3); }
 
 __device__ __forceinline__ gd_i16x4 lds_tr(const uint16_t* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gd_i16x4*)(p));
@@ -272,54 +268,85 @@ __device__ __forceinline__ gd_i16x8 fragment(const uint16_t* img, int x0, int s,
   }
 }
 
-// WM x WN waves, each of TM x TN blocks of 16 x 16
-template <typename E, int WM, int WN, int TM, int TN, bool AC, bool BC>
+// One operand's way into its LDS image of X rows (or columns) by 64 values of r.  A wave instruction moves 64 pieces
+// of 16 bytes to consecutive LDS positions, so the swizzle is applied to the source: position pos of a row holds
+// its chunk pos ^ swz.  Rows (columns) past the operand's end read its last one instead: their products land in
+// outputs that are not stored.
+template <int X, bool COL, int WAVES>
+struct Loader {
+  static constexpr int kInstr = X * 8 / 64 / WAVES;  // per wave and chunk
+  static_assert(kInstr * 64 * WAVES == X * 8, "the waves share an image evenly");
+  const uint16_t* src[kInstr];
+  int64_t step;  // from chunk to chunk
+  uint16_t* dst;  // within an image
+  __device__ __forceinline__ Loader(const uint16_t* p, int64_t ld, int x0, int end, int cols, int r0, int wave, int lane) {
+    step = COL ? kR * ld : kR;
+#pragma unroll
+    for (int h = 0; h < kInstr; ++h) {
+      const int piece = (wave + WAVES * h) * 64 + lane;
+      if (COL) {
+        const int r = piece / (X / 8), x = x0 + 8 * ((piece % (X / 8)) ^ col_swz<X>(r));
+        src[h] = p + int64_t(r0 + r) * ld + (x < cols ? x : cols - 8);
+      } else {
+        const int row = piece >> 3, x = x0 + row < end ? x0 + row : end - 1;
+        src[h] = p + int64_t(x) * ld + r0 + 8 * ((piece & 7) ^ row_swz(row));
+      }
+    }
+  }
+  __device__ __forceinline__ void issue(uint16_t* img, int wave) {
+#pragma unroll
+    for (int h = 0; h < kInstr; ++h) {
+      GD_LDS_DMA16(src[h], img + (wave + WAVES * h) * 512);
+      src[h] += step;
+    }
+  }
+};
+
+// the chunk of r that ends inside: through registers, zeros past the operand's end
+template <int X, bool COL, int WAVES>
+__device__ __forceinline__ void load_tail(uint16_t* img, const uint16_t* p, int64_t ld, int x0, int end, int cols, int r0,
+                                          int r_end) {
+#pragma unroll
+  for (int v = threadIdx.x; v < X * 8; v += 64 * WAVES) {
+    const int xi = COL ? 8 * (v % (X / 8)) : v >> 3, ri = COL ? v / (X / 8) : 8 * (v & 7);
+    const int x = x0 + xi, r = r0 + ri;
+    const bool ok = r < r_end && x < (COL ? cols : end);
+    const uint4 u = ok ? *reinterpret_cast<const uint4*>(p + (COL ? int64_t(r) * ld + x : int64_t(x) * ld + r))
+                       : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(img + (COL ? col_at<X>(ri, v % (X / 8)) : row_at(xi, v & 7))) = u;
+  }
+}
+
+// WM x WN waves, each of TM x TN blocks of 16 x 16; a ring of ST images, ST - 1 chunks of r in flight
+template <typename E, int WM, int WN, int TM, int TN, int ST, bool AC, bool BC>
 __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
-  constexpr int kThreads = 64 * WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
-  constexpr int kStage = (BM + BN) * kR, NA = BM * 8 / kThreads, NB = BN * 8 / kThreads;
+  constexpr int kWaves = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
+  constexpr int kStage = (BM + BN) * kR;
   constexpr int kPitch = 16 * TN + 4;  // floats: the epilogue's rows
-  static_assert(WM * WN * 16 * kPitch * 2 <= 2 * kStage, "the epilogue's staging fits");
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStage];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  static_assert(kWaves * 16 * kPitch * 2 <= ST * kStage, "the epilogue's staging fits");
+  __shared__ __attribute__((aligned(16))) uint16_t lds[ST * kStage];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / WN, wn = wave % WN;
   // the tiles of one part of r, n fastest, contiguous per XCD: they share rows of A and all of B in its L2
   const int L = xcd_remap(int(blockIdx.x), int(gridDim.x));
   const int tiles = int(gridDim.x) / p.splits;
   const int split = L / tiles, tile = L - split * tiles;
   const int m0 = tile / p.tiles_n * BM, n0 = tile % p.tiles_n * BN;
-  const int r_end = p.ra > p.rb ? p.ra : p.rb;
+  const int r_end = p.ra > p.rb ? p.ra : p.rb, r_both = p.ra < p.rb ? p.ra : p.rb;
   const int rb0 = split * p.r_per_split;
   const int re = rb0 + p.r_per_split < r_end ? rb0 + p.r_per_split : r_end;
+  const int rf = re < r_both ? re : r_both;
+  const int nfull = rf > rb0 ? (rf - rb0) / kR : 0;
 
-  uint4 ra[NA], rb[NB];
-  auto load = [&](int r0) {
-#pragma unroll
-    for (int h = 0; h < NA; ++h) {
-      const int v = tid + kThreads * h;
-      const int x = AC ? m0 + 8 * (v % (BM / 8)) : m0 + (v >> 3), r = r0 + (AC ? v / (BM / 8) : 8 * (v & 7));
-      const bool ok = r < p.ra && x < (AC ? p.ca : p.M);
-      ra[h] = ok ? *reinterpret_cast<const uint4*>(p.a + (AC ? r * p.lda + x : x * p.lda + r)) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      const int v = tid + kThreads * h;
-      const int x = BC ? n0 + 8 * (v % (BN / 8)) : n0 + (v >> 3), r = r0 + (BC ? v / (BN / 8) : 8 * (v & 7));
-      const bool ok = r < p.rb && x < (BC ? p.cb : p.N);
-      rb[h] = ok ? *reinterpret_cast<const uint4*>(p.b + (BC ? r * p.ldb + x : x * p.ldb + r)) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  auto stash = [&](uint16_t* img) {
-#pragma unroll
-    for (int h = 0; h < NA; ++h) {
-      const int v = tid + kThreads * h;
-      *reinterpret_cast<uint4*>(img + (AC ? col_at<BM>(v / (BM / 8), v % (BM / 8)) : row_at(v >> 3, v & 7))) = ra[h];
-    }
-#pragma unroll
-    for (int h = 0; h < NB; ++h) {
-      const int v = tid + kThreads * h;
-      *reinterpret_cast<uint4*>(img + BM * kR + (BC ? col_at<BN>(v / (BN / 8), v % (BN / 8)) : row_at(v >> 3, v & 7))) =
-          rb[h];
-    }
+  using LA = Loader<BM, AC, kWaves>;
+  using LB = Loader<BN, BC, kWaves>;
+  constexpr int kInstr = LA::kInstr + LB::kInstr;
+  LA la(p.a, p.lda, m0, p.M, p.ca, rb0, wave, lane);
+  LB lb(p.b, p.ldb, n0, p.N, p.cb, rb0, wave, lane);
+  auto issue = [&](int k) {
+    uint16_t* img = lds + k % ST * kStage;
+    la.issue(img, wave);
+    lb.issue(img + BM * kR, wave);
   };
 
   gd_f32x4 acc[TM][TN];
@@ -327,51 +354,94 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = gd_f32x4{0.f, 0.f, 0.f, 0.f};
-
-  if (rb0 < re) load(rb0);
-  for (int r0 = rb0, buf = 0; r0 < re; r0 += kR, buf ^= 1) {
-    uint16_t* img = lds + buf * kStage;
-    stash(img);
-    if (r0 + kR < re) load(r0 + kR);  // in flight during the products
-    gd_lds_barrier();                 // image complete; the other one was consumed an iteration ago
+  auto compute = [&](const uint16_t* img) {
 #pragma unroll
     for (int s = 0; s < kR / 32; ++s) {
       gd_i16x8 fa[TM], fb[TN];
 #pragma unroll
-      for (int i = 0; i < TM; ++i) fa[i] = fragment<BM, AC>(img, 16 * (wm * TM + i), s, lane);
-#pragma unroll
       for (int j = 0; j < TN; ++j) fb[j] = fragment<BN, BC>(img + BM * kR, 16 * (wn * TN + j), s, lane);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = fragment<BM, AC>(img, 16 * (wm * TM + i), s, lane);
       // transposed: lane (c, g) receives C[16 i + c][16 j + 4 g .. + 3], four values of a row
 #pragma unroll
       for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = E::mma(fb[j], fa[i], acc[i][j]);
     }
+  };
+
+#pragma unroll
+  for (int k = 0; k < ST - 1; ++k)
+    if (k < nfull) issue(k);
+  for (int k = 0; k < nfull; ++k) {
+    if (ST > 2 && nfull - 1 - k >= ST - 2)
+      gd_wait_vmcnt((ST - 2) * kInstr);
+    else if (ST > 3 && nfull - 1 - k == ST - 3)
+      gd_wait_vmcnt((ST > 3 ? ST - 3 : 0) * kInstr);
+    else
+      gd_wait_vmcnt(0);
+    gd_lds_barrier();  // chunk k has landed for every wave, and every wave has read chunk k - 1
+    if (k + ST - 1 < nfull) issue(k + ST - 1);
+    compute(lds + k % ST * kStage);
+  }
+  for (int r0 = rb0 + nfull * kR; r0 < re; r0 += kR) {  // (none of the ring is in flight)
+    __syncthreads();
+    load_tail<BM, AC, kWaves>(lds, p.a, p.lda, m0, p.M, p.ca, r0, p.ra < re ? p.ra : re);
+    load_tail<BN, BC, kWaves>(lds + BM * kR, p.b, p.ldb, n0, p.N, p.cb, r0, p.rb < re ? p.rb : re);
+    __syncthreads();
+    compute(lds);
   }
 
   // Each wave passes 16 rows at a time through its own LDS, so that a row leaves in 16-byte pieces of neighbouring
   // lanes; pitch 16 TN + 4: 16 rows' float4s, and the reads of 8 neighbouring columns, touch all banks once.
+  // A lane keeps its columns, so the bias is loaded once; the residual of the next 16 rows is under way meanwhile.
+  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes, kPasses = 16 / kRows;  // lanes per row, rows per pass
+  const int col = 8 * (lane % kLanes), n = n0 + 16 * wn * TN + col, left = p.N - n < 8 ? p.N - n : 8;
+  const bool whole = p.splits == 1;
+  float bias[8], res[kPasses][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+  if (whole && p.epi.bias && left > 0) ld8<E>(p.epi.bias, n, false, p.epi.bias_vec, left, bias);
+  auto row_of = [&](int i, int h) { return m0 + 16 * (wm * TM + i) + h * kRows + lane / kLanes; };
+  auto load_res = [&](int i) {
+#pragma unroll
+    for (int h = 0; h < kPasses; ++h) {
+      const int m = row_of(i, h);
+      if (m < p.M && left > 0)
+        ld8<E>(p.epi.res, m * p.epi.ldr + n, p.epi.res_f32, p.epi.res_vec, left, res[h]);
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < kPasses; ++h)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) res[h][j] = 0.f;
+  const bool has_res = whole && p.epi.res != nullptr;
+  if (has_res) load_res(0);
   __syncthreads();
   float* own = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
-  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes;  // lanes per row, rows per pass
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
 #pragma unroll
     for (int j = 0; j < TN; ++j)
       *reinterpret_cast<gd_f32x4*>(own + (lane & 15) * kPitch + 16 * j + 4 * (lane >> 4)) = acc[i][j];
     gd_wave_sync();
+    float now[kPasses][8];
 #pragma unroll
-    for (int h = 0; h < 16 / kRows; ++h) {
-      const int row = h * kRows + lane / kLanes, col = 8 * (lane % kLanes);
-      const int m = m0 + 16 * (wm * TM + i) + row, n = n0 + 16 * wn * TN + col;
+    for (int h = 0; h < kPasses; ++h)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[h][j] = res[h][j];
+    if (has_res && i + 1 < TM) load_res(i + 1);
+#pragma unroll
+    for (int h = 0; h < kPasses; ++h) {
+      const int row = h * kRows + lane / kLanes, m = row_of(i, h);
       const float4 u = *reinterpret_cast<const float4*>(own + row * kPitch + col);
       const float4 w = *reinterpret_cast<const float4*>(own + row * kPitch + col + 4);
       float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-      if (m < p.M && n < p.N) {
-        if (p.splits > 1)
-          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, p.N - n, v);
+      if (m < p.M && left > 0) {
+        if (whole)
+          epilogue8<E>(p.epi, m, n, p.N, bias, now[h], v);
         else
-          epilogue8<E>(p.epi, m, n, p.N, v);
+          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, left, v);
       }
     }
     gd_wave_sync();
@@ -395,7 +465,11 @@ __global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ p
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += u[j];
   }
-  epilogue8<E>(epi, m, n, N, v);
+  float b[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  const int left = N - n < 8 ? N - n : 8;
+  if (epi.bias) ld8<E>(epi.bias, n, false, epi.bias_vec, left, b);
+  if (epi.res) ld8<E>(epi.res, m * epi.ldr + n, epi.res_f32, epi.res_vec, left, r);
+  epilogue8<E>(epi, m, n, N, b, r, v);
 }
 
 // ---- dz = dy * act'(z), and parts of its column sums -------------------------------
@@ -503,9 +577,9 @@ Plan plan_of(int M, int N, int r) {
   Plan p;
   const int64_t big = div_up(M, 128) * div_up(N, 128), small = div_up(M, 64) * div_up(N, 64);
   p.tile = big >= 192 || (M > 64 && N > 64 && big * (r / 512) >= 192) ? 128 : 64;
-  const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64 or 128)
-  if (forced == 64 || forced == 128) p.tile = forced;
-  const int64_t tiles = p.tile == 128 ? big : small;
+  const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256)
+  if (forced == 64 || forced == 128 || forced == 256) p.tile = forced;
+  const int64_t tiles = p.tile == 256 ? div_up(M, 256) * div_up(N, 256) : p.tile == 128 ? big : small;
   int64_t s = tiles >= 192 ? 1 : 512 / tiles;
   const int64_t most = r / 256;
   s = s > most ? most : s;
@@ -525,10 +599,12 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.tiles_n = int(div_up(g.N, plan.tile));
   const int64_t grid = tm * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
-  if (plan.tile == 128)
-    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+  if (plan.tile == 256)
+    hipLaunchKernelGGL((linear_gemm<E, 2, 4, 8, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(512), 0, s, g);
+  else if (plan.tile == 128)
+    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   else
-    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 2, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((linear_gemm<E, 2, 2, 2, 2, 3, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   GD_LAUNCH_CHECK("linear_gemm");
   if (plan.splits > 1) {
     const int64_t blocks = div_up(int64_t(g.M) * ((g.N + 7) / 8), 256);

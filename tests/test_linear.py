@@ -31,7 +31,7 @@ def test_linear_act(emulated, m, k, n, act, dtype, residual, bias):
     lc.check(x, w, b, act, r, y, dy, grads)
 
 
-@pytest.mark.parametrize("tile", ["64", "128"])
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
 @pytest.mark.parametrize("m,k,n,act,dtype", [(150, 72, 136, "gelu", BF), (129, 200, 8, "none", HF),
                                              (1100, 8, 24, "relu", BF), (3, 1030, 16, "silu", BF)])
 def test_tiles(emulated, monkeypatch, tile, m, k, n, act, dtype):

@@ -29,7 +29,7 @@ def test_linear_act(m, k, n, act, dtype, residual, bias):
     lc.check(x, w, b, act, r, y, dy, grads)
 
 
-@pytest.mark.parametrize("tile", ["64", "128"])
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
 @pytest.mark.parametrize("m,k,n", [(300, 136, 264), (257, 513, 127), (5, 2048, 520), (4100, 72, 40)])
 def test_tiles(monkeypatch, tile, m, k, n):
     monkeypatch.setenv("GD_LINEAR_TILE", tile)
