@@ -84,6 +84,25 @@ def lib() -> ctypes.CDLL:
         return _lib
 
 
+_host = None        # the C++ host side (gdino_amd._host) ...
+_host_bound = None  # ... and the library whose entry points it holds
+_HOST_ENTRY_POINTS = ("gd_last_error", "gd_linear_forward_workspace_bytes", "gd_linear_forward",
+                      "gd_linear_backward_workspace_bytes", "gd_linear_backward", "gd_adamw_step",
+                      "gd_grad_norm_workspace_bytes", "gd_grad_norm")
+
+
+def host():
+    """The C++ host side of gdino_amd.linear and gdino_amd.optim (csrc/host/
+    host.cpp), calling the loaded library's entry points."""
+    global _host, _host_bound
+    handle = _lib if _lib is not None else lib()
+    if handle is not _host_bound:
+        from . import _host as module  # built beside the library (csrc/Makefile)
+        module.bind({n: ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _HOST_ENTRY_POINTS})
+        _host, _host_bound = module, handle
+    return _host
+
+
 def register(name: str, argtypes) -> None:
     """Declare the signature of an additional entry point (used by kernel
     modules that extend the ABI)."""

@@ -19,7 +19,6 @@ with ``args.optimizer = "adamw_hip"`` (``args.optimizer_state_bits`` 32 or 8).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -33,71 +32,28 @@ _lib.register("gd_adamw_step", [_i, _p, _p, _i, _p, _i, _p, _p, _p, _p, _p, _p, 
 _lib.register("gd_grad_norm", [_i, _p, _i, _p, _p, ctypes.c_size_t, _p, _p])
 
 BLOCK = 32  # elements of an 8-bit moment that share a scale
-_GRAD_TYPES = (_lib.GD_F32, _lib.GD_BF16)
-_U8, _E4M3, _E8M0 = 4, 5, 6  # _tensors.TYPES
-
-
-def _describe(tensors, written=False):
-    from . import _tensors  # built beside the library (csrc/Makefile)
-    return _tensors.describe(tensors if type(tensors) is list else list(tensors), written)
-
-
-def _guard(device: int):
-    """The launches go to the tensors' device, also where another is current."""
-    if device >= 0 and device != torch.cuda.current_device():
-        return torch.cuda.device(device)
-    return contextlib.nullcontext()
-
-
-def _check(what, name, got, n, device, types, sizes=None):
-    """One list's description against the call's: its length, place, layout, type and element counts."""
-    addr, size, kind, dev, dense = got
-    if len(addr) != 8 * n:
-        raise ValueError(f"{what}: {len(addr) // 8} {name} for {n} tensors")
-    if n and dev != device:
-        raise RuntimeError(f"{what}: {name} are not all on the device of the first tensor")
-    if not dense:
-        raise RuntimeError(f"{name} tensors have to be contiguous ({what})")
-    if n and kind not in types:
-        raise TypeError(f"gdino_amd {what}: unsupported or mixed dtypes of {name}")
-    if sizes is not None and size != sizes:
-        raise ValueError(f"{what}: {name} and the weights differ in their numbers of elements")
-    return addr
-
-
-def _scalar(what, name, t, device):
-    """The address of a one-element fp32 tensor on the call's device."""
-    if t.dtype != torch.float32 or t.numel() != 1:
-        raise TypeError(f"gdino_amd {what}: {name} is a one-element fp32 tensor, not {t.dtype} {tuple(t.shape)}")
-    if _describe([t])[3] != device:
-        raise RuntimeError(f"{what}: {name} is on {t.device}, the tensors are elsewhere")
-    return t.data_ptr()
 
 
 def grad_norm(grads) -> torch.Tensor:
     """sqrt of the sum of all squares of ``grads`` (contiguous, all fp32 or
     all bf16, on one device) -> 0-dim fp32 tensor.  No host synchronisation."""
-    grads = list(grads)
+    grads = grads if type(grads) is list else list(grads)
     if not grads:
         return torch.zeros(())
-    what = "grad_norm"
-    got = _describe(grads)
-    device = got[3]
-    _lib.require_device(grads[0], what=what)
-    addr = _check(what, "gradients", got, len(grads), device, _GRAD_TYPES)
-    fn = _lib.lib().gd_grad_norm_workspace_bytes
-    fn.restype, fn.argtypes = ctypes.c_size_t, [_i, _p]
-    nbytes = int(fn(len(grads), got[1]))
-    with _guard(device):
-        ws = torch.empty(nbytes // 8, dtype=torch.float64, device=grads[0].device)
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        _lib.call("gd_grad_norm", len(grads), got[1], got[2], addr, ws.data_ptr(), nbytes, out.data_ptr(),
-                  _lib.stream_of(out), nbytes=_elements(got) * (4 if got[2] == _lib.GD_F32 else 2))
+    if not _lib.on_device(grads[0]):
+        _lib.require_device(grads[0], what="grad_norm")
+    return _timed("gd_grad_norm", grads, 1, lambda: _lib.host().grad_norm(grads))
+
+
+def _timed(name, tensors, factor, call):
+    """call(), in the call timer's records where one is set: `factor` times the tensors' bytes."""
+    timer = _lib.call_timer
+    if timer is None:
+        return call()
+    start = timer.begin()
+    out = call()
+    timer.end(name, start, None, factor * sum(t.numel() * t.element_size() for t in tensors))
     return out
-
-
-def _elements(got):
-    return sum(memoryview(got[1]).cast("q")) if _lib.call_timer is not None else 0
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
@@ -120,63 +76,33 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     that is written must not overlap.  No host synchronisation: with the step
     counts and lr on the device the call can be captured and replayed."""
     what = "adamw_step"
-    params = list(params)
-    n = len(params)
-    got = _describe(params, True)
-    device = got[3]
-    if n:
+    params = params if type(params) is list else list(params)
+    if params and not _lib.on_device(params[0]):
         _lib.require_device(params[0], what=what)
-    pa = _check(what, "weights", got, n, device, (_lib.GD_F32,))
-    sizes = got[1]
-    g = _describe(grads)
-    ga = _check(what, "gradients", g, n, device, _GRAD_TYPES, sizes)
-    eight = exp_avg_scales is not None
-    if eight != (exp_avg_sq_scales is not None):
-        raise ValueError(f"{what}: moments in 8 bits have two lists of scales")
-    kinds = (_U8, _E4M3) if eight else (_lib.GD_F32,)
-    ma = _check(what, "exp_avgs", _describe(exp_avgs, True), n, device, kinds, sizes)
-    va = _check(what, "exp_avg_sqs", _describe(exp_avg_sqs, True), n, device, kinds, sizes)
-    msa = vsa = ca = sa = None
-    if eight:
-        blocks = memoryview(sizes).cast("q")
-        blocks = (ctypes.c_int64 * n)(*[-(-k // BLOCK) for k in blocks])
-        msa, vsa = (_check(what, name, _describe(x, True), n, device, (_U8, _E8M0), bytes(blocks))
-                    for name, x in (("exp_avg_scales", exp_avg_scales), ("exp_avg_sq_scales", exp_avg_sq_scales)))
-    if copies is not None:
-        ca = _check(what, "copies", _describe(copies, True), n, device, (_lib.GD_BF16,), sizes)
+    steps = None
     if isinstance(step, (list, tuple)):
-        steps = _describe(step)
-        sa = _check(what, "steps", steps, n, device, (_lib.GD_F32,))
-        if any(k != 1 for k in memoryview(steps[1]).cast("q")):
-            raise ValueError(f"{what}: a step count is one element")
-        step = 0
+        steps, step = step, 0
     elif not step >= 1:
         raise ValueError(f"{what}: step counts from 1, not {step}")
-    b1, b2 = (float(b) for b in betas)
+    b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
         raise ValueError(f"{what}: betas {betas}, eps {eps}, weight_decay {weight_decay}")
     lr_dev = None
-    if torch.is_tensor(lr) and not lr.is_cpu:
-        lr_dev, lr = _scalar(what, "lr", lr, device), 0.0
+    if torch.is_tensor(lr) and (steps is not None or not lr.is_cpu):
+        lr_dev, lr = lr, 0.0
     lr = float(lr)
     if not (lr >= 0.0 and math.isfinite(lr)):
         raise ValueError(f"{what}: lr {lr}")
-    norm = None
-    if total_norm is not None:
-        if not max_norm > 0.0:
-            raise ValueError(f"{what}: total_norm comes with a positive max_norm")
-        norm = _scalar(what, "total_norm", total_norm, device)
-    if n == 0:
-        return
-    with _guard(device):
-        _lib.call("gd_adamw_step", n, sizes, pa, g[2], ga, 8 if eight else 32, ma, va, msa, vsa, ca, sa, float(step),
-                  lr, lr_dev, b1, b2, float(eps), float(weight_decay), norm, float(max_norm), int(seed) & 0xFFFFFFFF,
-                  _lib.stream_of(params[0]),
-                  nbytes=_elements(got) * (8 + (4 if g[2] == _lib.GD_F32 else 2) + (4.125 if eight else 16)
-                                           + (0 if ca is None else 2)))
-    torch.autograd.graph.increment_version(params)
-    if copies is not None:
-        torch.autograd.graph.increment_version(copies)
+    if total_norm is not None and not max_norm > 0.0:
+        raise ValueError(f"{what}: total_norm comes with a positive max_norm")
+
+    def call():
+        _lib.host().adamw_step(params, grads, exp_avgs, exp_avg_sqs, exp_avg_scales, exp_avg_sq_scales, copies, steps,
+                               step, lr_dev, lr, b1, b2, eps, weight_decay, total_norm, max_norm,
+                               int(seed) & 0xFFFFFFFF)
+
+    # (the weights are read and written; the other lists count by the moments' share of that)
+    _timed("gd_adamw_step", params, 4.03 if exp_avg_scales is not None else 7.0, call)
 
 
 def adamw_state(p: torch.Tensor, bits: int = 32) -> dict:
