@@ -135,8 +135,21 @@ __device__ __forceinline__ void lds_dma16(const void* src, void* dst) {
                : "v"(src), "s"(lds_addr)
                : "memory");
 }
+// the same from a wave-uniform base and a 32-bit byte offset per lane (half the address registers) to a
+// wave-uniform byte position of an LDS array
+template <typename T>
+__device__ __forceinline__ void lds_dma16_at(const void* base, uint32_t offset, T* lds, uint32_t at) {
+  const uint32_t lds_addr = __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)(lds))) + at);
+  uint32_t keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep)
+               : "v"(offset), "s"(base), "s"(lds_addr)
+               : "memory");
+}
 }  // namespace
 #define GD_LDS_DMA16(src, dst) ::gd::lds_dma16((src), (dst))
+#define GD_LDS_DMA16_AT(base, offset, lds, at) ::gd::lds_dma16_at((base), (offset), (lds), (at))
 #endif
 // s_waitcnt vmcnt(N) (expcnt, lgkmcnt left open), N < 64; and a bare
 // s_barrier, which unlike __syncthreads() does not wait vmcnt(0) first

@@ -84,7 +84,7 @@ struct Forward {
 Forward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, int act, const Tensor& r, bool want_z,
                        at::IntArrayRef lead) {
   const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
-  TORCH_CHECK_VALUE(m <= (1 << 30) && k <= (1 << 30) && n <= (1 << 30), "linear_act: too large");
+  TORCH_CHECK_VALUE(m <= (1 << 30) && k <= (1 << 22) && n <= (1 << 22), "linear_act: over 2^30 rows or 2^22 features");
   const auto like = x.options().requires_grad(false);
   Forward f;
   c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());

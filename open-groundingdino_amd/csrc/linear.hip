@@ -19,6 +19,7 @@
 #include "gd_common.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace gd {
 namespace {
@@ -31,6 +32,16 @@ typedef float gd_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 gd_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
 
+// acc += a b with acc held in accumulation registers, which 256 of the compiler's own products would move
+// back and forth; their results are read only after GD_MMA_WAIT8 (a matrix instruction's result takes up to 18
+// cycles, which the compiler does not see in assembly)
+#ifndef GD_MMA_IN_PLACE
+#define GD_MMA_IN_PLACE(name, acc, a, b, E) asm volatile(name " %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b))
+#define GD_MMA_WAIT8(nops, r)                                                                              \
+  asm volatile(nops : "+a"((r)[0]), "+a"((r)[1]), "+a"((r)[2]), "+a"((r)[3]), "+a"((r)[4]), "+a"((r)[5]), \
+                     "+a"((r)[6]), "+a"((r)[7]))
+#endif
+
 // the two 16-bit types
 struct Bf16 {
   static __device__ __forceinline__ float up(uint16_t h) { return bf16_to_f32(h); }
@@ -38,6 +49,9 @@ struct Bf16 {
   static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b),
                                                    c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ void mma_in(gd_f32x4& c, gd_i16x8 a, gd_i16x8 b) {
+    GD_MMA_IN_PLACE("v_mfma_f32_16x16x32_bf16", c, a, b, Bf16);
   }
 };
 struct Fp16 {
@@ -49,6 +63,9 @@ struct Fp16 {
   static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gd_f16x8, a), __builtin_bit_cast(gd_f16x8, b), c,
                                                   0, 0, 0);
+  }
+  static __device__ __forceinline__ void mma_in(gd_f32x4& c, gd_i16x8 a, gd_i16x8 b) {
+    GD_MMA_IN_PLACE("v_mfma_f32_16x16x32_f16", c, a, b, Fp16);
   }
 };
 
@@ -229,12 +246,30 @@ struct Gemm {
   int ra, rb;    // extents of r in memory; the shorter operand counts as zero beyond (rows: multiples of 8)
   int ca, cb;    // columns in memory of a "columns" operand, multiples of 8
   int splits, r_per_split;  // r_per_split: a multiple of kR
-  int tiles_n;
+  int tiles_m, tiles_n, group;  // group: see tile_of
   float* part;   // splits > 1: [splits][M][N]
   Epi epi;
 };
 
 constexpr int kR = 64;  // values of r per staged chunk
+
+// A workgroup's tile.  Each XCD gets a contiguous range of the parts' tiles (its L2 is its own), in bands of `group`
+// rows of tiles, down the band first: the tiles that run at one time on an XCD then cover a block of the output
+// that is about square, and need the fewest rows of A and B from beyond its L2.
+struct Tile {
+  int m, n, split;
+};
+__device__ __forceinline__ Tile tile_of(const Gemm& p) {
+  const int L = xcd_remap(int(blockIdx.x), int(gridDim.x));
+  const int tiles = p.tiles_m * p.tiles_n;
+  Tile t;
+  t.split = L / tiles;
+  const int i = L - t.split * tiles, band = i / (p.group * p.tiles_n), first = band * p.group;
+  const int high = p.tiles_m - first < p.group ? p.tiles_m - first : p.group, j = i - first * p.tiles_n;
+  t.m = first + j % high;
+  t.n = j / high;
+  return t;
+}
 
 // Offset of 16-byte chunk ch of row r in an LDS image.  Rows image [x][64 r]: 128-byte rows; 16 lanes read the same
 // chunk of 16 consecutive rows, so the chunk index is xored with row / 2: with the row's parity that is every one of
@@ -276,29 +311,32 @@ template <int X, bool COL, int WAVES>
 struct Loader {
   static constexpr int kInstr = X * 8 / 64 / WAVES;  // per wave and chunk
   static_assert(kInstr * 64 * WAVES == X * 8, "the waves share an image evenly");
-  const uint16_t* src[kInstr];
-  int64_t step;  // from chunk to chunk
-  uint16_t* dst;  // within an image
+  const uint16_t* base;      // of the tile and chunk, the same for every lane
+  int64_t step;              // from chunk to chunk
+  uint32_t offset[kInstr];   // bytes (the host keeps row pitches below kMaxPitch)
   __device__ __forceinline__ Loader(const uint16_t* p, int64_t ld, int x0, int end, int cols, int r0, int wave, int lane) {
     step = COL ? kR * ld : kR;
+    base = p + (COL ? int64_t(r0) * ld + x0 : int64_t(x0) * ld + r0);
 #pragma unroll
     for (int h = 0; h < kInstr; ++h) {
       const int piece = (wave + WAVES * h) * 64 + lane;
       if (COL) {
-        const int r = piece / (X / 8), x = x0 + 8 * ((piece % (X / 8)) ^ col_swz<X>(r));
-        src[h] = p + int64_t(r0 + r) * ld + (x < cols ? x : cols - 8);
+        const int r = piece / (X / 8), x = 8 * ((piece % (X / 8)) ^ col_swz<X>(r));
+        offset[h] = uint32_t(r * uint32_t(ld) + (x0 + x < cols ? x : cols - 8 - x0)) * 2;
       } else {
-        const int row = piece >> 3, x = x0 + row < end ? x0 + row : end - 1;
-        src[h] = p + int64_t(x) * ld + r0 + 8 * ((piece & 7) ^ row_swz(row));
+        const int row = piece >> 3, x = x0 + row < end ? row : end - 1 - x0;
+        offset[h] = (uint32_t(x) * uint32_t(ld) + 8 * ((piece & 7) ^ row_swz(row))) * 2;
       }
     }
   }
-  __device__ __forceinline__ void issue(uint16_t* img, int wave) {
+  // piece h of the chunk to the image at byte `at` of the LDS array
+  __device__ __forceinline__ void issue(uint16_t* lds, uint32_t at, int wave, int h) const {
+    GD_LDS_DMA16_AT(base, offset[h], lds, at + uint32_t(wave + WAVES * h) * 1024);
+  }
+  __device__ __forceinline__ void issue(uint16_t* lds, uint32_t at, int wave) {
 #pragma unroll
-    for (int h = 0; h < kInstr; ++h) {
-      GD_LDS_DMA16(src[h], img + (wave + WAVES * h) * 512);
-      src[h] += step;
-    }
+    for (int h = 0; h < kInstr; ++h) issue(lds, at, wave, h);
+    base += step;
   }
 };
 
@@ -317,6 +355,55 @@ __device__ __forceinline__ void load_tail(uint16_t* img, const uint16_t* p, int6
   }
 }
 
+// A wave's TM x TN blocks to memory: 16 rows at a time through its own LDS (own), so that a row leaves in 16-byte
+// pieces of neighbouring lanes; pitch 16 TN + 4: 16 rows' float4s, and the reads of 8 neighbouring columns, touch
+// all banks once.  A lane keeps its columns, so the bias is loaded once; the residual of its next row is under way
+// meanwhile.  m0, n0: the wave's corner.
+template <typename E, int TM, int TN>
+__device__ __forceinline__ void store_tile(const Gemm& p, const gd_f32x4 (&acc)[TM][TN], float* own, int m0, int n0,
+                                           int split, int lane) {
+  constexpr int kPitch = 16 * TN + 4;
+  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes, kPasses = 16 / kRows;  // lanes per row, rows per pass
+  const int col = 8 * (lane % kLanes), n = n0 + col, left = p.N - n < 8 ? p.N - n : 8;
+  const bool whole = p.splits == 1;
+  float bias[8], res[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = res[j] = 0.f;
+  if (whole && p.epi.bias && left > 0) ld8<E>(p.epi.bias, n, false, p.epi.bias_vec, left, bias);
+  const bool has_res = whole && p.epi.res != nullptr;
+  auto load_res = [&](int m) {
+    if (has_res && m < p.M && left > 0) ld8<E>(p.epi.res, m * p.epi.ldr + n, p.epi.res_f32, p.epi.res_vec, left, res);
+  };
+  m0 += lane / kLanes;  // this lane's first row; it takes every kRows-th
+  load_res(m0);
+  __syncthreads();  // the images have been read
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      *reinterpret_cast<gd_f32x4*>(own + (lane & 15) * kPitch + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+    gd_wave_sync();
+#pragma unroll 1
+    for (int h = 0; h < kPasses; ++h) {
+      const int row = h * kRows + lane / kLanes, m = m0 + 16 * i + h * kRows;
+      float now[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now[j] = res[j];
+      load_res(m + kRows);  // of the next pass
+      const float4 u = *reinterpret_cast<const float4*>(own + row * kPitch + col);
+      const float4 w = *reinterpret_cast<const float4*>(own + row * kPitch + col + 4);
+      float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+      if (m < p.M && left > 0) {
+        if (whole)
+          epilogue8<E>(p.epi, m, n, p.N, bias, now, v);
+        else
+          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, left, v);
+      }
+    }
+    gd_wave_sync();
+  }
+}
+
 // WM x WN waves, each of TM x TN blocks of 16 x 16; a ring of ST images, ST - 1 chunks of r in flight
 template <typename E, int WM, int WN, int TM, int TN, int ST, bool AC, bool BC>
 __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
@@ -327,11 +414,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[ST * kStage];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / WN, wn = wave % WN;
-  // the tiles of one part of r, n fastest, contiguous per XCD: they share rows of A and all of B in its L2
-  const int L = xcd_remap(int(blockIdx.x), int(gridDim.x));
-  const int tiles = int(gridDim.x) / p.splits;
-  const int split = L / tiles, tile = L - split * tiles;
-  const int m0 = tile / p.tiles_n * BM, n0 = tile % p.tiles_n * BN;
+  const Tile t = tile_of(p);
+  const int m0 = t.m * BM, n0 = t.n * BN, split = t.split;
   const int r_end = p.ra > p.rb ? p.ra : p.rb, r_both = p.ra < p.rb ? p.ra : p.rb;
   const int rb0 = split * p.r_per_split;
   const int re = rb0 + p.r_per_split < r_end ? rb0 + p.r_per_split : r_end;
@@ -344,9 +428,9 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   LA la(p.a, p.lda, m0, p.M, p.ca, rb0, wave, lane);
   LB lb(p.b, p.ldb, n0, p.N, p.cb, rb0, wave, lane);
   auto issue = [&](int k) {
-    uint16_t* img = lds + k % ST * kStage;
-    la.issue(img, wave);
-    lb.issue(img + BM * kR, wave);
+    const uint32_t at = uint32_t(k % ST) * (2 * kStage);
+    la.issue(lds, at, wave);
+    lb.issue(lds, at + 2 * BM * kR, wave);
   };
 
   gd_f32x4 acc[TM][TN];
@@ -392,60 +476,129 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
     compute(lds);
   }
 
-  // Each wave passes 16 rows at a time through its own LDS, so that a row leaves in 16-byte pieces of neighbouring
-  // lanes; pitch 16 TN + 4: 16 rows' float4s, and the reads of 8 neighbouring columns, touch all banks once.
-  // A lane keeps its columns, so the bias is loaded once; the residual of the next 16 rows is under way meanwhile.
-  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes, kPasses = 16 / kRows;  // lanes per row, rows per pass
-  const int col = 8 * (lane % kLanes), n = n0 + 16 * wn * TN + col, left = p.N - n < 8 ? p.N - n : 8;
-  const bool whole = p.splits == 1;
-  float bias[8], res[kPasses][8];
+  store_tile<E, TM, TN>(p, acc, reinterpret_cast<float*>(lds) + wave * 16 * kPitch, m0 + 16 * wm * TM, n0 + 16 * wn * TN,
+                        split, lane);
+}
+
+// 256 x 256 tiles of 4 waves, 128 x 128 each, one per SIMD: the largest wave tile its 512 registers allow, since LDS is
+// what the matrix cores compete for (128 KB are read and 64 KB written per chunk of 64 values of r; 8 waves of 128 x
+// 64 read 192 KB and wait for each other: 444 us at 16384 x 4096 x 4096, the products and reads alone 286, the
+// loads alone 299).  A phase multiplies half a chunk whose fragments are in registers; between its products the next
+// half's fragments are read and the loads issued, so nothing waits but for the barrier in the middle of a chunk.
+// LDS holds a ring of 5 images of one operand each, in the order A0 B0 A1 B1 A2 ...: when chunk k has been read, its two
+// images take B of chunk k + 2, needed first, and A of chunk k + 3.
+template <typename E, bool AC, bool BC>
+__global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
+  constexpr int T = 8, kWaves = 4, BX = 256, kImg = BX * kR, kRing = 5;
+  constexpr int kPitch = 16 * T + 4;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kRing * kImg];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+  const Tile t = tile_of(p);
+  const int m0 = t.m * BX, n0 = t.n * BX, split = t.split;
+  const int r_end = p.ra > p.rb ? p.ra : p.rb, r_both = p.ra < p.rb ? p.ra : p.rb;
+  const int rb0 = split * p.r_per_split;
+  const int re = rb0 + p.r_per_split < r_end ? rb0 + p.r_per_split : r_end;
+  const int rf = re < r_both ? re : r_both;
+  const int nfull = rf > rb0 ? (rf - rb0) / kR : 0;
+
+  using Load = Loader<BX, AC, kWaves>;  // 8 instructions a wave and image
+  Load la(p.a, p.lda, m0, p.M, p.ca, rb0, wave, lane);
+  Loader<BX, BC, kWaves> lb(p.b, p.ldb, n0, p.N, p.cb, rb0, wave, lane);
+  static_assert(Load::kInstr == T, "one instruction per row of blocks");
+
+  gd_f32x4 acc[T][T];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) bias[j] = 0.f;
-  if (whole && p.epi.bias && left > 0) ld8<E>(p.epi.bias, n, false, p.epi.bias_vec, left, bias);
-  auto row_of = [&](int i, int h) { return m0 + 16 * (wm * TM + i) + h * kRows + lane / kLanes; };
-  auto load_res = [&](int i) {
+  for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int h = 0; h < kPasses; ++h) {
-      const int m = row_of(i, h);
-      if (m < p.M && left > 0)
-        ld8<E>(p.epi.res, m * p.epi.ldr + n, p.epi.res_f32, p.epi.res_vec, left, res[h]);
-    }
+    for (int j = 0; j < T; ++j) acc[i][j] = gd_f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Frags {
+    gd_i16x8 a[T], b[T];
   };
+  // image q of the ring, as its byte in LDS; its operand's fragment i, half s
+  auto wrap = [](int q) { return q >= kRing ? q - kRing : q; };
+  auto read1 = [&](Frags& f, int qa, int s, int i) {
+    f.a[i] = fragment<BX, AC>(lds + qa * kImg, 16 * (wm * T + i), s, lane);
+    f.b[i] = fragment<BX, BC>(lds + wrap(qa + 1) * kImg, 16 * (wn * T + i), s, lane);
+  };
+  auto multiply1 = [&](const Frags& f, int i) {
 #pragma unroll
-  for (int h = 0; h < kPasses; ++h)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) res[h][j] = 0.f;
-  const bool has_res = whole && p.epi.res != nullptr;
-  if (has_res) load_res(0);
-  __syncthreads();
-  float* own = reinterpret_cast<float*>(lds) + wave * 16 * kPitch;
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-      *reinterpret_cast<gd_f32x4*>(own + (lane & 15) * kPitch + 16 * j + 4 * (lane >> 4)) = acc[i][j];
-    gd_wave_sync();
-    float now[kPasses][8];
-#pragma unroll
-    for (int h = 0; h < kPasses; ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) now[h][j] = res[h][j];
-    if (has_res && i + 1 < TM) load_res(i + 1);
-#pragma unroll
-    for (int h = 0; h < kPasses; ++h) {
-      const int row = h * kRows + lane / kLanes, m = row_of(i, h);
-      const float4 u = *reinterpret_cast<const float4*>(own + row * kPitch + col);
-      const float4 w = *reinterpret_cast<const float4*>(own + row * kPitch + col + 4);
-      float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-      if (m < p.M && left > 0) {
-        if (whole)
-          epilogue8<E>(p.epi, m, n, p.N, bias, now[h], v);
-        else
-          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, left, v);
-      }
+    for (int j = 0; j < T; ++j) E::mma_in(acc[i][j], f.b[j], f.a[i]);
+  };
+
+  Frags f0, f1;
+  if (nfull > 0) {
+    la.issue(lds, 0, wave);
+    lb.issue(lds, 2 * kImg, wave);
+    if (nfull > 1) {
+      la.issue(lds, 4 * kImg, wave);
+      lb.issue(lds, 6 * kImg, wave);
     }
-    gd_wave_sync();
+    if (nfull > 2) {
+      la.issue(lds, 8 * kImg, wave);
+      gd_wait_vmcnt(3 * T);
+    } else {
+      gd_wait_vmcnt(0);
+    }
+    gd_raw_barrier();
+#pragma unroll
+    for (int i = 0; i < T; ++i) read1(f0, 0, 0, i);
+    // one chunk; q: its A's image.  MORE: chunks k + 2 and k + 3 exist
+    auto chunk = [&](int k, int q, auto MORE) {
+      constexpr bool kMore = decltype(MORE)::value;
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        read1(f1, q, 1, i);
+        multiply1(f0, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // chunk k + 1 has landed, all but A of chunk k + 2; and chunk k has been read
+      if (kMore || k + 2 < nfull)
+        gd_wait_vmcnt(T);
+      else
+        gd_wait_vmcnt(0);
+      gd_lds_barrier();
+      const int qn = k + 1 < nfull ? wrap(q + 2) : q;  // (the last chunk's is read again, for nothing)
+      const uint32_t to_b = uint32_t(q) * (2 * kImg), to_a = uint32_t(wrap(q + 1)) * (2 * kImg);
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        read1(f0, qn, 0, i);
+        if (i < T / 2) {
+          if (kMore || k + 2 < nfull) {
+            lb.issue(lds, to_b, wave, 2 * i);
+            lb.issue(lds, to_b, wave, 2 * i + 1);
+          }
+        } else if (kMore) {
+          la.issue(lds, to_a, wave, 2 * i - T);
+          la.issue(lds, to_a, wave, 2 * i - T + 1);
+        }
+        multiply1(f1, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      la.base += la.step;
+      lb.base += lb.step;
+    };
+    int k = 0, q = 0;
+    for (; k + 3 < nfull; ++k, q = wrap(q + 2)) chunk(k, q, std::true_type());
+    for (; k < nfull; ++k, q = wrap(q + 2)) chunk(k, q, std::false_type());
   }
+  for (int r0 = rb0 + nfull * kR; r0 < re; r0 += kR) {
+    __syncthreads();
+    load_tail<BX, AC, kWaves>(lds, p.a, p.lda, m0, p.M, p.ca, r0, p.ra < re ? p.ra : re);
+    load_tail<BX, BC, kWaves>(lds + kImg, p.b, p.ldb, n0, p.N, p.cb, r0, p.rb < re ? p.rb : re);
+    __syncthreads();
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int i = 0; i < T; ++i) read1(f0, 0, s, i);
+#pragma unroll
+      for (int i = 0; i < T; ++i) multiply1(f0, i);
+    }
+  }
+  GD_MMA_WAIT8("s_nop 15\n\ts_nop 7", acc[0]);
+#pragma unroll
+  for (int i = 1; i < T; ++i) GD_MMA_WAIT8("", acc[i]);
+  store_tile<E, T, T>(p, acc, reinterpret_cast<float*>(lds) + wave * 16 * kPitch, m0 + 16 * wm * T, n0 + 16 * wn * T,
+                      split, lane);
 }
 
 // the parts added in order, then the epilogue; a thread per 8 columns
@@ -563,7 +716,10 @@ __global__ void __launch_bounds__(256) linear_pack(const uint16_t* __restrict__ 
 int pad8(int n) { return (n + 7) / 8 * 8; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-bool packed(const void* p, int64_t ld, int cols) { return !(aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0); }
+constexpr int64_t kMaxPitch = int64_t(1) << 22;  // 256 rows' offsets fit 32 bits
+bool packed(const void* p, int64_t ld, int cols) {
+  return !(aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxPitch);
+}
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Tiles and parts of one product.  128 x 128 where that alone makes three quarters of a workgroup per CU, or where
@@ -578,8 +734,8 @@ Plan plan_of(int M, int N, int r) {
   const int64_t big = div_up(M, 128) * div_up(N, 128), small = div_up(M, 64) * div_up(N, 64);
   p.tile = big >= 192 || (M > 64 && N > 64 && big * (r / 512) >= 192) ? 128 : 64;
   const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256)
-  if (forced == 64 || forced == 128 || forced == 256) p.tile = forced;
-  const int64_t tiles = p.tile == 256 ? div_up(M, 256) * div_up(N, 256) : p.tile == 128 ? big : small;
+  if (forced == 64 || forced == 128 || forced >= 255) p.tile = forced;
+  const int64_t tiles = p.tile >= 255 ? div_up(M, 256) * div_up(N, 256) : p.tile == 128 ? big : small;
   int64_t s = tiles >= 192 ? 1 : 512 / tiles;
   const int64_t most = r / 256;
   s = s > most ? most : s;
@@ -595,11 +751,15 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.splits = plan.splits;
   g.r_per_split = plan.r_per_split;
   g.part = static_cast<float*>(part);
-  const int64_t tm = div_up(g.M, plan.tile);
-  g.tiles_n = int(div_up(g.N, plan.tile));
-  const int64_t grid = tm * g.tiles_n * plan.splits;
+  const int tile = plan.tile == 255 ? 256 : plan.tile;
+  g.tiles_m = int(div_up(g.M, tile));
+  g.tiles_n = int(div_up(g.N, tile));
+  g.group = env_int("GD_LINEAR_GROUP", tile >= 256 ? 4 : 8);
+  const int64_t grid = int64_t(g.tiles_m) * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
   if (plan.tile == 256)
+    hipLaunchKernelGGL((linear_gemm256<E, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+  else if (plan.tile == 255)
     hipLaunchKernelGGL((linear_gemm<E, 2, 4, 8, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(512), 0, s, g);
   else if (plan.tile == 128)
     hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
@@ -678,8 +838,8 @@ gd_status check_shape(int dtype, int act, int M, int K, int N) {
   GD_REQUIRE(dtype == GD_BF16 || dtype == GD_F16, "linear: bf16 or fp16 operands");
   GD_REQUIRE(act >= kNone && act <= kSilu, "linear: activation %d", act);
   GD_REQUIRE(M >= 0 && K > 0 && N > 0, "linear: M=%d K=%d N=%d", M, K, N);
-  // (tile origins and chunk ends stay in int, padded extents too)
-  GD_REQUIRE(M <= (1 << 30) && K <= (1 << 30) && N <= (1 << 30), "linear: M=%d K=%d N=%d", M, K, N);
+  // (tile origins and chunk ends stay in int; features are a row's pitch)
+  GD_REQUIRE(M <= (1 << 30) && K <= kMaxPitch && N <= kMaxPitch, "linear: M=%d K=%d N=%d (K, N up to 2^22)", M, K, N);
   return GD_OK;
 }
 

@@ -463,8 +463,14 @@ inline int __ffsll(long long v) { return __builtin_ffsll(v); }
 #define __builtin_amdgcn_s_waitcnt(imm) ((void)(imm))  // memory is synchronous here
 #define gd_opaque_i32(x) (x)  // gd_common.h: a register-allocation hint only
 #define GD_LDS_DMA16(src, dst) ::gd_emu::lds_dma16((const void*)(src), (void*)(dst))
+#define GD_LDS_DMA16_AT(base, offset, lds, at) \
+  ::gd_emu::lds_dma16((const char*)(base) + (offset), (void*)((char*)(lds) + (at)))
+// csrc/linear.hip's in-place products and the wait for their results
+#define GD_MMA_IN_PLACE(name, acc, a, b, E) ((acc) = E::mma((a), (b), (acc)))
+#define GD_MMA_WAIT8(nops, r) ((void)(r))
 // compiler scheduling hints: no semantics to emulate
 #define __builtin_amdgcn_sched_barrier(mask) ((void)(mask))
+#define __builtin_amdgcn_s_setprio(level) ((void)(level))
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) ::gd_emu::ds_read_tr16_b64((const void*)(uintptr_t)(p))
 #define __builtin_amdgcn_ds_swizzle(v, pattern) ::gd_emu::ds_swizzle((v), (pattern))
 #define __builtin_amdgcn_update_dpp(old, src, ctrl, rm, bm, bc) \
