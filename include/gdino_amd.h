@@ -622,31 +622,36 @@ gd_status gd_grad_norm(int tensors, const int64_t* numel, int dtype, const uint6
 /* ------------------------------------------------------------------------ */
 /*
  *   y[M, N] = act(x[M, K] W[N, K]^T + bias[N]) + residual[M, N]
- * x, W, bias of `dtype` (bf16 / fp16), rows ldx / ldw elements apart, of any
- * alignment of their element and any M >= 0, K, N >= 1; accumulated, activated
- * and added in fp32, rounded once.  residual: NULL, or of `dtype` or fp32; y has its
- * type, or `dtype` without one.  act: 0 none, 1 ReLU, 2 GELU (erf), 3 GELU
- * (tanh form), 4 SiLU.  z: NULL, or [M][ldz] of `dtype` (16-byte aligned, ldz a
- * multiple of 8 and >= N) that receives x W^T + bias for the backward; what pads a
- * row to 8 values is zero. */
-size_t gd_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int K, int N);
+ * x, W, bias of `dtype` (bf16 / fp16); accumulated, activated and added in fp32,
+ * rounded once.  Any M >= 0 and K, N >= 1 (up to 2^22).  Rows of x and W, ldx / ldw elements
+ * apart, are read in 16-byte pieces: 16-byte aligned, a pitch of a multiple of 8,
+ * and K a multiple of 8 or, with `padded`, rows whose ends hold zeros up to one.
+ * gd_linear_readable says whether rows are so; gd_linear_pack copies two matrices
+ * of `cols` columns (rows_b 0: one) to such rows, pad8(cols) apart.
+ * residual: NULL, or of `dtype` or fp32; y has its type, or `dtype` without one.
+ * act: 0 none, 1 ReLU, 2 GELU (erf), 3 GELU (tanh form), 4 SiLU.  z: NULL, or
+ * [M][ldz] of `dtype` (16-byte aligned, ldz a multiple of 8 and >= N) that receives
+ * x W^T + bias for the backward; what pads a row to 8 values is zero. */
+int gd_linear_readable(const void* rows, int64_t ld, int cols, int padded);
+gd_status gd_linear_pack(const void* a, int64_t lda, int rows_a, const void* b, int64_t ldb, int rows_b, int cols,
+                         void* a_out, void* b_out, gd_stream_t stream);
+size_t gd_linear_forward_workspace_bytes(int M, int K, int N);
 gd_status gd_linear_forward(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
                             int act, const void* residual, int residual_dtype, int64_t ldr, int M, int K, int N,
-                            void* y, int y_dtype, int64_t ldy, void* z, int64_t ldz, void* workspace,
+                            void* y, int y_dtype, int64_t ldy, void* z, int64_t ldz, int padded, void* workspace,
                             size_t workspace_bytes, gd_stream_t stream);
 /*
  * dz = dy * act'(z), dx[M, K] = dz W, dw[N, K] = dz^T x, db[N] = sum over rows of
  * dz (fp32 sums of unrounded dz; dz is rounded to `dtype` for the products).
  * dy: of `dtype` or fp32.  z as the forward wrote it, or of a ReLU without a
- * residual its y; unused without an activation.  dx, dw, db: NULL where not
- * wanted; dx of dx_dtype, dw (contiguous) and db of param_dtype: `dtype` or fp32.
+ * residual its y; unused without an activation.  x, W: as in the forward.  dx, dw, db:
+ * NULL where not wanted; dx of dx_dtype, dw (contiguous) and db of param_dtype: `dtype` or fp32.
  * M >= 1.  Both calls can be captured into a graph. */
-size_t gd_linear_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int K, int N,
-                                          int dx, int dw, int db);
+size_t gd_linear_backward_workspace_bytes(int M, int K, int N, int dx, int dw, int db);
 gd_status gd_linear_backward(int dtype, int act, const void* dy, int dy_dtype, int64_t lddy, const void* z, int64_t ldz,
                              const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int K, int N, void* dx,
-                             int dx_dtype, int64_t lddx, void* dw, void* db, int param_dtype, void* workspace,
-                             size_t workspace_bytes, gd_stream_t stream);
+                             int dx_dtype, int64_t lddx, void* dw, void* db, int param_dtype, int padded,
+                             void* workspace, size_t workspace_bytes, gd_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Runtime                                                                   */

@@ -34,6 +34,8 @@ using at::Tensor;
 // ------------------------------------------------------------------ the library
 struct Api {
   decltype(&gd_last_error) last_error;
+  decltype(&gd_linear_readable) linear_readable;
+  decltype(&gd_linear_pack) linear_pack;
   decltype(&gd_linear_forward_workspace_bytes) linear_forward_bytes;
   decltype(&gd_linear_forward) linear_forward;
   decltype(&gd_linear_backward_workspace_bytes) linear_backward_bytes;
@@ -77,12 +79,13 @@ Tensor rows_of(const Tensor& t) {
 }
 
 struct Forward {
-  Tensor y, z;
+  Tensor y, z, x, w;  // x, w: as the kernels read them, K wide or padded to 8
 };
 
 // x [M, K], w [N, K], r [M, N]: rows; y of `lead`'s dimensions, its last one N
-Forward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, int act, const Tensor& r, bool want_z,
+Forward linear_forward(const Tensor& x0, const Tensor& w0, const Tensor& b, int act, const Tensor& r, bool want_z,
                        at::IntArrayRef lead) {
+  Tensor x = x0, w = w0;
   const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
   TORCH_CHECK_VALUE(m <= (1 << 30) && k <= (1 << 22) && n <= (1 << 22), "linear_act: over 2^30 rows or 2^22 features");
   const auto like = x.options().requires_grad(false);
@@ -90,16 +93,29 @@ Forward linear_forward(const Tensor& x, const Tensor& w, const Tensor& b, int ac
   c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end());
   shape.back() = n;
   f.y = at::empty(shape, r.defined() ? like.dtype(r.scalar_type()) : like);
+  f.x = x;
+  f.w = w;
   if (m == 0) return f;
   if (want_z) f.z = at::empty({m, (n + 7) / 8 * 8}, like);
   const c10::DeviceGuard guard(x.device());
-  const size_t bytes = api.linear_forward_bytes(data(x), x.stride(0), data(w), w.stride(0), m, k, n);
+  const bool pack_x = !api.linear_readable(data(x), x.stride(0), k, 0), pack_w = !api.linear_readable(data(w), w.stride(0), k, 0);
+  if (pack_x || pack_w) {
+    // (the copies also serve the backward)
+    const int64_t k8 = (k + 7) / 8 * 8;
+    if (pack_x) f.x = at::empty({m, k8}, like);
+    if (pack_w) f.w = at::empty({n, k8}, like);
+    run("gd_linear_pack", api.linear_pack(data(x), x.stride(0), pack_x ? m : 0, data(w), w.stride(0), pack_w ? n : 0, k,
+                                          mut(f.x), mut(f.w), stream_of(x)));
+    x = f.x;
+    w = f.w;
+  }
+  const size_t bytes = api.linear_forward_bytes(m, k, n);
   const Tensor ws = workspace(bytes, x);
   const int code = code_of(x.scalar_type());
   run("gd_linear_forward",
       api.linear_forward(code, data(x), x.stride(0), data(w), w.stride(0), data(b), act, data(r),
                          r.defined() ? code_of(r.scalar_type()) : code, r.defined() ? r.stride(0) : 0, m, k, n, mut(f.y),
-                         code_of(f.y.scalar_type()), n, mut(f.z), f.z.defined() ? f.z.stride(0) : 0, mut(ws), bytes,
+                         code_of(f.y.scalar_type()), n, mut(f.z), f.z.defined() ? f.z.stride(0) : 0, 1, mut(ws), bytes,
                          stream_of(x)));
   return f;
 }
@@ -116,7 +132,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const Tensor x2 = rows_of(xc);
     const Forward f = linear_forward(x2, wc, bc ? *bc : Tensor(), int(act), r, wants && act != 0 && !by_y,
                                      x.sizes());
-    ctx->save_for_backward({x2, wc, by_y ? f.y : f.z});
+    ctx->save_for_backward({f.x, f.w, by_y ? f.y : f.z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["x"] = x.sizes().vec();
     ctx->saved_data["types"] = std::vector<int64_t>{int64_t(x.scalar_type()), int64_t(weight.scalar_type())};
@@ -136,7 +152,8 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const auto given = ctx->saved_data["given"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = given[0] && ctx->needs_input_grad(2), want_r = given[1] && ctx->needs_input_grad(2 + given[0]);
-    const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
+    const auto shape = ctx->saved_data["x"].toIntVector();
+    const int64_t m = x.size(0), k = shape.back(), n = w.size(0);
     const auto xt = at::ScalarType(types[0]), wt = at::ScalarType(types[1]);
     const auto like = x.options().requires_grad(false);
     Tensor dx, dw, db;
@@ -151,15 +168,14 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       Tensor z = saved[2];
       if (z.defined()) z = z.dim() == 2 ? z : z.reshape({m, -1});
       const c10::DeviceGuard guard(x.device());
-      const size_t bytes = api.linear_backward_bytes(data(x), x.stride(0), data(w), w.stride(0), m, k, n, want_x, want_w,
-                                                     want_b);
+      const size_t bytes = api.linear_backward_bytes(m, k, n, want_x, want_w, want_b);
       const Tensor ws = workspace(bytes, x);
       run("gd_linear_backward",
           api.linear_backward(code_of(x.scalar_type()), act, data(g), code_of(g.scalar_type()), g.stride(0), data(z),
                               z.defined() ? z.stride(0) : 0, data(x), x.stride(0), data(w), w.stride(0), m, k, n, mut(dx),
-                              code_of(xt), k, mut(dw), mut(db), code_of(wt), mut(ws), bytes, stream_of(x)));
+                              code_of(xt), k, mut(dw), mut(db), code_of(wt), 1, mut(ws), bytes, stream_of(x)));
     }
-    if (want_x) out[0] = dx.view(ctx->saved_data["x"].toIntVector());
+    if (want_x) out[0] = dx.view(shape);
     out[1] = dw;
     if (given[0]) out[2] = db;
     if (want_r) out[3] = dy;
@@ -305,6 +321,8 @@ PyObject* py_bind(PyObject*, PyObject* addresses) {
     };
     Api a;
     get("gd_last_error", a.last_error);
+    get("gd_linear_readable", a.linear_readable);
+    get("gd_linear_pack", a.linear_pack);
     get("gd_linear_forward_workspace_bytes", a.linear_forward_bytes);
     get("gd_linear_forward", a.linear_forward);
     get("gd_linear_backward_workspace_bytes", a.linear_backward_bytes);

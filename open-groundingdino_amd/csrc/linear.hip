@@ -88,6 +88,11 @@ __device__ __forceinline__ float normal_cdf(float z, float* bell) {
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_of(-z)); }
 
 constexpr float kTanhC = 0.79788456080286536f, kTanhA = 0.044715f;
+// sigmoid(2 c (z + a z^3)), which is (1 + tanh(c (z + a z^3))) / 2, as 1 / (1 + 2^(z (p + q z^2)))
+__device__ __forceinline__ float tanh_gate(float z) {
+  constexpr float p = -2.f * kTanhC * 1.4426950408889634f, q = p * kTanhA;
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * (p + q * (z * z))));
+}
 
 // (the switch around the 8 values: a uniform branch each, not eight)
 __device__ __forceinline__ void activate8(float v[8], int act) {
@@ -103,9 +108,9 @@ __device__ __forceinline__ void activate8(float v[8], int act) {
         v[j] *= normal_cdf(v[j], &bell);
       }
       break;
-    case kGeluTanh:  // (1 + tanh u) / 2 = sigmoid(2 u)
+    case kGeluTanh:
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= sigmoid(2.f * kTanhC * (v[j] + kTanhA * v[j] * v[j] * v[j]));
+      for (int j = 0; j < 8; ++j) v[j] *= tanh_gate(v[j]);
       break;
     case kSilu:
 #pragma unroll
@@ -133,7 +138,7 @@ __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
     case kGeluTanh:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float q = sigmoid(2.f * kTanhC * (z[j] + kTanhA * z[j] * z[j] * z[j]));
+        const float q = tanh_gate(z[j]);
         d[j] *= q + 2.f * z[j] * q * (1.f - q) * kTanhC * (1.f + 3.f * kTanhA * z[j] * z[j]);
       }
       break;
@@ -221,9 +226,8 @@ struct Epi {
 
 // 8 values of a row: bias b and residual r were loaded before (zeros where there is none)
 template <typename E>
-__device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N, const float b[8], const float r[8],
-                                          float v[8]) {
-  const int left = N - n < 8 ? N - n : 8;
+__device__ __forceinline__ void epilogue8(const Epi& e, int act, int64_t m, int n, int left, const float b[8],
+                                          const float r[8], float v[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] += b[j];
   if (e.z) {
@@ -232,7 +236,7 @@ __device__ __forceinline__ void epilogue8(const Epi& e, int64_t m, int n, int N,
     for (int j = 0; j < 8; ++j) z[j] = j < left ? v[j] : 0.f;
     st8<E>(e.z, m * e.ldz + n, false, true, 8, z);
   }
-  activate8(v, e.act);
+  activate8(v, act);
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] += r[j];
   st8<E>(e.y, m * e.ldy + n, e.y_f32, e.y_vec, left, v);
@@ -355,50 +359,152 @@ __device__ __forceinline__ void load_tail(uint16_t* img, const uint16_t* p, int6
   }
 }
 
-// A wave's TM x TN blocks to memory: 16 rows at a time through its own LDS (own), so that a row leaves in 16-byte
-// pieces of neighbouring lanes; pitch 16 TN + 4: 16 rows' float4s, and the reads of 8 neighbouring columns, touch
-// all banks once.  A lane keeps its columns, so the bias is loaded once; the residual of its next row is under way
-// meanwhile.  m0, n0: the wave's corner.
-template <typename E, int TM, int TN>
+// A wave's TM x TN blocks to memory, through its own LDS in TM / GI parts, so that a row leaves in 16-byte pieces of
+// neighbouring lanes and the loop over the rows is short code with several rows under way (the accumulators can
+// only be addressed by unrolled code).  Pitch 16 TN + 4 floats: 16 rows' float4s, and the reads of 8 neighbouring
+// columns, touch all banks once.
+template <int TN>
+constexpr int store_pitch() { return 16 * TN + 4; }
+template <int TN>
+constexpr int store_floats(int gi) { return 16 * gi * store_pitch<TN>(); }  // of one wave
+
+// The residual of B rows, asked for before the previous ones are used: it comes from far, and y may be anywhere,
+// so the compiler would not move a load before a store.  Without a branch in between: the second half of an fp32
+// row is of a 16-bit one the same piece again, and rows past the end are the last one.
+template <int B>
+struct Residual {
+  uint4 a[B], b[B];
+  __device__ __forceinline__ void load(const Gemm& p, int m, int step, int n) {
+    const char* const from = static_cast<const char*>(p.epi.res);
+    const int64_t size = p.epi.res_f32 ? 4 : 2;
+#pragma unroll
+    for (int h = 0; h < B; ++h) {
+      const int row = m + h * step < p.M ? m + h * step : p.M - 1;
+      const uint4* q = reinterpret_cast<const uint4*>(from + (row * p.epi.ldr + n) * size);
+      a[h] = q[0];
+      b[h] = q[p.epi.res_f32 ? 1 : 0];
+    }
+  }
+  template <typename E>
+  __device__ __forceinline__ void get(const Gemm& p, int h, float r[8]) const {
+    union {
+      uint4 u[2];
+      uint16_t h16[8];
+      float f[8];
+    } raw;
+    raw.u[0] = a[h];
+    raw.u[1] = b[h];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = p.epi.res_f32 ? raw.f[j] : E::up(raw.h16[j]);
+  }
+};
+
+template <int TN>
+constexpr int rows_per_pass() { return 64 / (2 * TN); }  // 2 TN lanes per row
+template <int TN, int GI>
+constexpr int batch() { return 16 * GI / rows_per_pass<TN>() < 4 ? 16 * GI / rows_per_pass<TN>() : 4; }
+
+// 16 GI rows in LDS, whose corner in the output is m0, n0; a lane keeps its 8 columns.  next: the residual's rows from m0
+// on, where `ahead` says that it is loaded this way.
+template <typename E, int TN, int GI, int ACT>
+__device__ __forceinline__ void store_rows(const Gemm& p, const float* own, Residual<batch<TN, GI>()>& next,
+                                           bool ahead, int m0, int n0,
+                                           int lane) {
+  constexpr int kLanes = 2 * TN, kRows = rows_per_pass<TN>(), kBatch = batch<TN, GI>();
+  constexpr int kBatches = 16 * GI / (kRows * kBatch);
+  const int col = 8 * (lane % kLanes), n = n0 + col, left = p.N - n < 8 ? p.N - n : 8;
+  if (left <= 0) return;
+  float bias[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) bias[j] = 0.f;
+  if (p.epi.bias) ld8<E>(p.epi.bias, n, false, p.epi.bias_vec, left, bias);
+#pragma unroll 1
+  for (int b = 0; b < kBatches; ++b) {
+    const int row0 = b * kBatch * kRows + lane / kLanes;
+    Residual<kBatch> now;
+    if (ahead) {
+      now = next;
+      if (m0 + row0 + kBatch * kRows < p.M) next.load(p, m0 + row0 + kBatch * kRows, kRows, n);
+    }
+#pragma unroll
+    for (int h = 0; h < kBatch; ++h) {
+      const int row = row0 + h * kRows, m = m0 + row;
+      if (m < p.M) {
+        float res[8];
+        if (ahead) {
+          now.template get<E>(p, h, res);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) res[j] = 0.f;
+          if (p.epi.res) ld8<E>(p.epi.res, m * p.epi.ldr + n, p.epi.res_f32, p.epi.res_vec, left, res);
+        }
+        const float4 u = *reinterpret_cast<const float4*>(own + row * store_pitch<TN>() + col);
+        const float4 w = *reinterpret_cast<const float4*>(own + row * store_pitch<TN>() + col + 4);
+        float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+        epilogue8<E>(p.epi, ACT, m, n, left, bias, res, v);
+      }
+    }
+  }
+}
+
+// the same without an epilogue: a gradient, or a part of a split sum
+template <typename E, int TN>
+__device__ __forceinline__ void store_plain(const Gemm& p, const float* own, int rows, int m0, int n0, int split, int lane) {
+  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes;
+  const int col = 8 * (lane % kLanes), n = n0 + col, left = p.N - n < 8 ? p.N - n : 8;
+  if (left <= 0) return;
+  const bool whole = p.splits == 1;
+  void* const to = whole ? p.epi.y : static_cast<void*>(p.part + int64_t(split) * p.M * p.N);
+  const int64_t ld = whole ? p.epi.ldy : p.N;
+  const bool f32 = !whole || p.epi.y_f32, vec = whole ? p.epi.y_vec : (p.N & 3) == 0;
+  const int end = p.M - m0 < rows ? p.M - m0 : rows;
+#pragma unroll 4
+  for (int row = lane / kLanes; row < end; row += kRows) {
+    const float4 u = *reinterpret_cast<const float4*>(own + row * store_pitch<TN>() + col);
+    const float4 w = *reinterpret_cast<const float4*>(own + row * store_pitch<TN>() + col + 4);
+    const float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+    st8<E>(to, (m0 + row) * ld + n, f32, vec, left, v);
+  }
+}
+
+// own: the wave's LDS, its part of the images, which every wave has read
+template <typename E, int TM, int TN, int GI, bool LAYER>
 __device__ __forceinline__ void store_tile(const Gemm& p, const gd_f32x4 (&acc)[TM][TN], float* own, int m0, int n0,
                                            int split, int lane) {
-  constexpr int kPitch = 16 * TN + 4;
-  constexpr int kLanes = 2 * TN, kRows = 64 / kLanes, kPasses = 16 / kRows;  // lanes per row, rows per pass
-  const int col = 8 * (lane % kLanes), n = n0 + col, left = p.N - n < 8 ? p.N - n : 8;
-  const bool whole = p.splits == 1;
-  float bias[8], res[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) bias[j] = res[j] = 0.f;
-  if (whole && p.epi.bias && left > 0) ld8<E>(p.epi.bias, n, false, p.epi.bias_vec, left, bias);
-  const bool has_res = whole && p.epi.res != nullptr;
-  auto load_res = [&](int m) {
-    if (has_res && m < p.M && left > 0) ld8<E>(p.epi.res, m * p.epi.ldr + n, p.epi.res_f32, p.epi.res_vec, left, res);
-  };
-  m0 += lane / kLanes;  // this lane's first row; it takes every kRows-th
-  load_res(m0);
-  __syncthreads();  // the images have been read
-#pragma unroll
-  for (int i = 0; i < TM; ++i) {
-#pragma unroll
-    for (int j = 0; j < TN; ++j)
-      *reinterpret_cast<gd_f32x4*>(own + (lane & 15) * kPitch + 16 * j + 4 * (lane >> 4)) = acc[i][j];
-    gd_wave_sync();
+  static_assert(TM % GI == 0, "whole parts");
+  Residual<batch<TN, GI>()> next;
+  // (uniform: whole pieces of 8 columns, so that no lane needs another path)
+  const bool ahead = LAYER && p.splits == 1 && p.epi.res && p.epi.res_vec && (p.N & 7) == 0;
+  if (ahead) {
+    const int n = n0 + 8 * (lane % (2 * TN));
+    if (n < p.N && m0 < p.M) next.load(p, m0 + lane / (2 * TN), rows_per_pass<TN>(), n);
+  }
+  __syncthreads();
+  // (one copy of the rows' code, which is long; the accumulators are picked by comparison)
 #pragma unroll 1
-    for (int h = 0; h < kPasses; ++h) {
-      const int row = h * kRows + lane / kLanes, m = m0 + 16 * i + h * kRows;
-      float now[8];
+  for (int part = 0; part < TM / GI; ++part) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) now[j] = res[j];
-      load_res(m + kRows);  // of the next pass
-      const float4 u = *reinterpret_cast<const float4*>(own + row * kPitch + col);
-      const float4 w = *reinterpret_cast<const float4*>(own + row * kPitch + col + 4);
-      float v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-      if (m < p.M && left > 0) {
-        if (whole)
-          epilogue8<E>(p.epi, m, n, p.N, bias, now, v);
-        else
-          st8<E>(p.part, (int64_t(split) * p.M + m) * p.N + n, true, (p.N & 3) == 0, left, v);
+    for (int q = 0; q < TM / GI; ++q)
+      if (q == part) {
+#pragma unroll
+        for (int i = 0; i < GI; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j)
+            *reinterpret_cast<gd_f32x4*>(own + (16 * i + (lane & 15)) * store_pitch<TN>() + 16 * j + 4 * (lane >> 4)) =
+                acc[q * GI + i][j];
       }
+    gd_wave_sync();
+    const int m = m0 + 16 * GI * part;
+    if (LAYER && p.splits == 1) {
+      switch (p.epi.act) {
+        case kRelu: store_rows<E, TN, GI, kRelu>(p, own, next, ahead, m, n0, lane); break;
+        case kGelu: store_rows<E, TN, GI, kGelu>(p, own, next, ahead, m, n0, lane); break;
+        case kGeluTanh: store_rows<E, TN, GI, kGeluTanh>(p, own, next, ahead, m, n0, lane); break;
+        case kSilu: store_rows<E, TN, GI, kSilu>(p, own, next, ahead, m, n0, lane); break;
+        default: store_rows<E, TN, GI, kNone>(p, own, next, ahead, m, n0, lane); break;
+      }
+    } else {
+      store_plain<E, TN>(p, own, 16 * GI, m, n0, split, lane);
     }
     gd_wave_sync();
   }
@@ -409,8 +515,8 @@ template <typename E, int WM, int WN, int TM, int TN, int ST, bool AC, bool BC>
 __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   constexpr int kWaves = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
   constexpr int kStage = (BM + BN) * kR;
-  constexpr int kPitch = 16 * TN + 4;  // floats: the epilogue's rows
-  static_assert(kWaves * 16 * kPitch * 2 <= ST * kStage, "the epilogue's staging fits");
+  constexpr int kOwn = store_floats<TN>(2);
+  static_assert(kWaves * kOwn * 2 <= ST * kStage, "the output's way through LDS fits");
   __shared__ __attribute__((aligned(16))) uint16_t lds[ST * kStage];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / WN, wn = wave % WN;
@@ -476,8 +582,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
     compute(lds);
   }
 
-  store_tile<E, TM, TN>(p, acc, reinterpret_cast<float*>(lds) + wave * 16 * kPitch, m0 + 16 * wm * TM, n0 + 16 * wn * TN,
-                        split, lane);
+  store_tile<E, TM, TN, 2, !AC && !BC>(p, acc, reinterpret_cast<float*>(lds) + wave * kOwn, m0 + 16 * wm * TM,
+                                       n0 + 16 * wn * TN, split, lane);
 }
 
 // 256 x 256 tiles of 4 waves, 128 x 128 each, one per SIMD: the largest wave tile its 512 registers allow, since LDS is
@@ -485,12 +591,14 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
 // 64 read 192 KB and wait for each other: 444 us at 16384 x 4096 x 4096, the products and reads alone 286, the
 // loads alone 299).  A phase multiplies half a chunk whose fragments are in registers; between its products the next
 // half's fragments are read and the loads issued, so nothing waits but for the barrier in the middle of a chunk.
-// LDS holds a ring of 5 images of one operand each, in the order A0 B0 A1 B1 A2 ...: when chunk k has been read, its two
-// images take B of chunk k + 2, needed first, and A of chunk k + 3.
+// LDS holds a ring of 5 images of one operand each, in the order A0 B0 A1 B1 A2 ...: A of chunk k + 2 is loaded in the
+// first phase of chunk k, to the image that B of chunk k - 1 left, B of chunk k + 2 in the second, to that of A of
+// chunk k: one load per 8 products, all the time.
 template <typename E, bool AC, bool BC>
 __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   constexpr int T = 8, kWaves = 4, BX = 256, kImg = BX * kR, kRing = 5;
-  constexpr int kPitch = 16 * T + 4;
+  constexpr int kOwn = store_floats<T>(4);
+  static_assert(kWaves * kOwn * 2 <= kRing * kImg, "the output's way through LDS fits");
   __shared__ __attribute__((aligned(16))) uint16_t lds[kRing * kImg];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave >> 1, wn = wave & 1;
@@ -534,44 +642,34 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
       la.issue(lds, 4 * kImg, wave);
       lb.issue(lds, 6 * kImg, wave);
     }
-    if (nfull > 2) {
-      la.issue(lds, 8 * kImg, wave);
-      gd_wait_vmcnt(3 * T);
-    } else {
+    if (nfull > 1)
+      gd_wait_vmcnt(2 * T);
+    else
       gd_wait_vmcnt(0);
-    }
     gd_raw_barrier();
 #pragma unroll
     for (int i = 0; i < T; ++i) read1(f0, 0, 0, i);
-    // one chunk; q: its A's image.  MORE: chunks k + 2 and k + 3 exist
+    // one chunk; q: its A's image.  MORE: chunk k + 2 exists
     auto chunk = [&](int k, int q, auto MORE) {
       constexpr bool kMore = decltype(MORE)::value;
+      const uint32_t to_a = uint32_t(wrap(q + 4)) * (2 * kImg), to_b = uint32_t(q) * (2 * kImg);
 #pragma unroll
       for (int i = 0; i < T; ++i) {
         read1(f1, q, 1, i);
+        if (kMore) la.issue(lds, to_a, wave, i);
         multiply1(f0, i);
         __builtin_amdgcn_sched_barrier(0);
       }
-      // chunk k + 1 has landed, all but A of chunk k + 2; and chunk k has been read
-      if (kMore || k + 2 < nfull)
-        gd_wait_vmcnt(T);
+      if (kMore)
+        gd_wait_vmcnt(T);  // chunk k + 1 has landed, A of chunk k + 2 may be under way
       else
         gd_wait_vmcnt(0);
-      gd_lds_barrier();
+      gd_lds_barrier();  // and chunk k has been read
       const int qn = k + 1 < nfull ? wrap(q + 2) : q;  // (the last chunk's is read again, for nothing)
-      const uint32_t to_b = uint32_t(q) * (2 * kImg), to_a = uint32_t(wrap(q + 1)) * (2 * kImg);
 #pragma unroll
       for (int i = 0; i < T; ++i) {
         read1(f0, qn, 0, i);
-        if (i < T / 2) {
-          if (kMore || k + 2 < nfull) {
-            lb.issue(lds, to_b, wave, 2 * i);
-            lb.issue(lds, to_b, wave, 2 * i + 1);
-          }
-        } else if (kMore) {
-          la.issue(lds, to_a, wave, 2 * i - T);
-          la.issue(lds, to_a, wave, 2 * i - T + 1);
-        }
+        if (kMore) lb.issue(lds, to_b, wave, i);
         multiply1(f1, i);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -579,7 +677,7 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
       lb.base += lb.step;
     };
     int k = 0, q = 0;
-    for (; k + 3 < nfull; ++k, q = wrap(q + 2)) chunk(k, q, std::true_type());
+    for (; k + 2 < nfull; ++k, q = wrap(q + 2)) chunk(k, q, std::true_type());
     for (; k < nfull; ++k, q = wrap(q + 2)) chunk(k, q, std::false_type());
   }
   for (int r0 = rb0 + nfull * kR; r0 < re; r0 += kR) {
@@ -597,8 +695,8 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   GD_MMA_WAIT8("s_nop 15\n\ts_nop 7", acc[0]);
 #pragma unroll
   for (int i = 1; i < T; ++i) GD_MMA_WAIT8("", acc[i]);
-  store_tile<E, T, T>(p, acc, reinterpret_cast<float*>(lds) + wave * 16 * kPitch, m0 + 16 * wm * T, n0 + 16 * wn * T,
-                      split, lane);
+  store_tile<E, T, T, 4, !AC && !BC>(p, acc, reinterpret_cast<float*>(lds) + wave * kOwn, m0 + 16 * wm * T,
+                                     n0 + 16 * wn * T, split, lane);
 }
 
 // the parts added in order, then the epilogue; a thread per 8 columns
@@ -622,7 +720,7 @@ __global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ p
   const int left = N - n < 8 ? N - n : 8;
   if (epi.bias) ld8<E>(epi.bias, n, false, epi.bias_vec, left, b);
   if (epi.res) ld8<E>(epi.res, m * epi.ldr + n, epi.res_f32, epi.res_vec, left, r);
-  epilogue8<E>(epi, m, n, N, b, r, v);
+  epilogue8<E>(epi, epi.act, m, n, left, b, r, v);
 }
 
 // ---- dz = dy * act'(z), and parts of its column sums -------------------------------
@@ -646,18 +744,26 @@ __global__ void __launch_bounds__(256) linear_dact(const Dact p) {
   const int left = p.N - n < 8 ? p.N - n : 8;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   if (left > 0) {
-#pragma unroll 2
-    for (int64_t m = begin + at; m < end; m += rows) {
-      float d[8];
-      ld8<E>(p.dy, m * p.lddy + n, p.dy_f32, p.dy_vec, left, d);
-      if (p.z) {
-        float z[8];
-        ld8<E>(p.z, m * p.ldz + n, false, p.z_vec, left, z);
-        slope8(d, z, p.act);  // (beyond `left` both are zero)
-      }
-      if (p.dz) st8<E>(p.dz, m * p.lddz + n, false, true, 8, d);
+    // (4 rows are loaded before the first is stored, which the compiler could not do by itself: dz may be anywhere)
+    constexpr int kRowsAhead = 4;
+    for (int64_t m = begin + at; m < end; m += kRowsAhead * rows) {
+      float d[kRowsAhead][8], z[kRowsAhead][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] += d[j];
+      for (int h = 0; h < kRowsAhead; ++h) {
+        const int64_t row = m + h * rows < end ? m + h * rows : end - 1;
+        ld8<E>(p.dy, row * p.lddy + n, p.dy_f32, p.dy_vec, left, d[h]);
+        if (p.z) ld8<E>(p.z, row * p.ldz + n, false, p.z_vec, left, z[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < kRowsAhead; ++h) {
+        const int64_t row = m + h * rows;
+        if (row < end) {
+          if (p.z) slope8(d[h], z[h], p.act);  // (beyond `left` both are zero)
+          if (p.dz) st8<E>(p.dz, row * p.lddz + n, false, true, 8, d[h]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[j] += d[h][j];
+        }
+      }
     }
   }
   if (!p.sums) return;
@@ -696,20 +802,28 @@ __global__ void __launch_bounds__(256) linear_colsum(const float* __restrict__ s
   }
 }
 
-// ---- rows that are not 16-byte aligned, copied with their ends filled with zeros ------
-__global__ void __launch_bounds__(256) linear_pack(const uint16_t* __restrict__ src, int64_t ld, int rows, int cols,
-                                                   uint16_t* __restrict__ dst, int per_row) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= int64_t(rows) * per_row) return;
-  const int64_t r = i / per_row;
-  const int c = int(i - r * per_row) * 8;
+// ---- rows that are not 16-byte aligned, copied with their ends filled with zeros; two matrices in one launch ------
+struct Pack {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int64_t ld[2], pieces[2];  // pieces: of 8 values, of the whole matrix (0: none)
+  int cols, per_row;
+};
+__global__ void __launch_bounds__(256) linear_pack(const Pack p) {
+  int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  const int which = i >= p.pieces[0];
+  if (which) i -= p.pieces[0];
+  if (i >= p.pieces[which]) return;
+  const int64_t r = i / p.per_row;
+  const int c = int(i - r * p.per_row) * 8;
+  const uint16_t* src = p.src[which] + r * p.ld[which] + c;
   union {
     uint4 u;
     uint16_t h[8];
   } w;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w.h[j] = c + j < cols ? src[r * ld + c + j] : uint16_t(0);
-  *reinterpret_cast<uint4*>(dst + i * 8) = w.u;
+  for (int j = 0; j < 8; ++j) w.h[j] = c + j < p.cols ? src[j] : uint16_t(0);
+  *reinterpret_cast<uint4*>(p.dst[which] + i * 8) = w.u;
 }
 
 // ---------------------------------------------------------------------------- host
@@ -717,31 +831,49 @@ int pad8(int n) { return (n + 7) / 8 * 8; }
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 constexpr int64_t kMaxPitch = int64_t(1) << 22;  // 256 rows' offsets fit 32 bits
-bool packed(const void* p, int64_t ld, int cols) {
-  return !(aligned(p, 16) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxPitch);
+// whether a product can read these rows as they are
+bool readable(const void* p, int64_t ld, int cols, bool padded) {
+  return aligned(p, 16) && ld % 8 == 0 && (cols % 8 == 0 || (padded && ld >= pad8(cols))) && ld <= kMaxPitch;
 }
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Tiles and parts of one product.  128 x 128 where that alone makes three quarters of a workgroup per CU, or where
-// r is long enough to be split to it; else 64 x 64, which has four times the workgroups.  r is split while two
-// workgroups per CU are not reached and each part keeps 256 values of r.
+// Tile and parts of one product: the cheapest by a model of what was measured (us, 16-bit, 64 values of r at a time).
+// A round is as many tiles as run at once (1, 2 or 3 workgroups per CU, by their LDS); it costs `base` (the first loads
+// and the output) and `chunk` per 64 values of r, `alone` where a CU has one workgroup only:
+//   256 x 256  16384 x 4096 x 4096 in 4 rounds of 64 chunks: 425 us.  Only where 8 tiles or more share each operand's
+//              chunk: it waits for one chunk at a time, which has to come from L2 (44446 x 2048 x 256: 100 us, by 128s 59)
+//   128 x 128  the same 490 us in 8 rounds; 8400 x 1536 x 384 in one, 198 workgroups: 22 us
+//   64 x 64    900 x 256 x 2048 in one round of 480: 6.1 us (by 128s 8.7)
+// Parts of a split sum are written and read once more, in fp32 at about 4 TB/s, by a further launch.
 struct Plan {
   int tile, splits, r_per_split;
   size_t bytes;
 };
 Plan plan_of(int M, int N, int r) {
-  Plan p;
-  const int64_t big = div_up(M, 128) * div_up(N, 128), small = div_up(M, 64) * div_up(N, 64);
-  p.tile = big >= 192 || (M > 64 && N > 64 && big * (r / 512) >= 192) ? 128 : 64;
+  struct Kind {
+    int tile, slots;
+    double chunk, alone, base;
+  };
+  constexpr Kind kinds[] = {{256, 256, 1.5, 1.5, 12.0}, {128, 512, 0.86, 0.65, 6.0}, {64, 768, 0.47, 0.35, 3.6}};
   const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256)
-  if (forced == 64 || forced == 128 || forced >= 255) p.tile = forced;
-  const int64_t tiles = p.tile >= 255 ? div_up(M, 256) * div_up(N, 256) : p.tile == 128 ? big : small;
-  int64_t s = tiles >= 192 ? 1 : 512 / tiles;
-  const int64_t most = r / 256;
-  s = s > most ? most : s;
-  s = s < 1 ? 1 : s;
-  p.r_per_split = int(div_up(div_up(r, s), kR) * kR);
-  p.splits = int(div_up(r, p.r_per_split));
+  const int64_t chunks = div_up(r, kR);
+  Plan p = {};
+  double best = 1e30;
+  for (const Kind& k : kinds) {
+    const int64_t tm = div_up(M, k.tile), tn = div_up(N, k.tile);
+    if (forced ? forced != k.tile : (k.tile == 256 && (tm < 8 || tn < 8))) continue;
+    for (int64_t s = 1; s == 1 || (s <= 64 && chunks / s >= 4); s *= 2) {
+      const int64_t part = div_up(chunks, s), parts = div_up(chunks, part), blocks = tm * tn * parts;
+      double cost = double(div_up(blocks, k.slots)) * (double(part) * (blocks <= 256 ? k.alone : k.chunk) + k.base);
+      if (parts > 1) cost += 5.0 + double(parts) * M * N * 8.0 / 4e6;
+      if (cost < best) {
+        best = cost;
+        p.tile = k.tile;
+        p.splits = int(parts);
+        p.r_per_split = int(part * kR);
+      }
+    }
+  }
   p.bytes = p.splits > 1 ? align256(size_t(p.splits) * M * N * sizeof(float)) : 0;
   return p;
 }
@@ -751,16 +883,13 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.splits = plan.splits;
   g.r_per_split = plan.r_per_split;
   g.part = static_cast<float*>(part);
-  const int tile = plan.tile == 255 ? 256 : plan.tile;
-  g.tiles_m = int(div_up(g.M, tile));
-  g.tiles_n = int(div_up(g.N, tile));
-  g.group = env_int("GD_LINEAR_GROUP", tile >= 256 ? 4 : 8);
+  g.tiles_m = int(div_up(g.M, plan.tile));
+  g.tiles_n = int(div_up(g.N, plan.tile));
+  g.group = plan.tile == 256 ? 4 : 8;  // (32 or 64 workgroups per XCD at a time)
   const int64_t grid = int64_t(g.tiles_m) * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
   if (plan.tile == 256)
     hipLaunchKernelGGL((linear_gemm256<E, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
-  else if (plan.tile == 255)
-    hipLaunchKernelGGL((linear_gemm<E, 2, 4, 8, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(512), 0, s, g);
   else if (plan.tile == 128)
     hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   else
@@ -775,31 +904,13 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   return GD_OK;
 }
 
-// an operand's rows: as they are, or packed into the workspace
+// an operand's rows; `padded`: their ends are filled with zeros up to a multiple of 8
 struct Rows {
   const uint16_t* p;
   int64_t ld;
   int cols;  // readable, a multiple of 8
 };
-gd_status rows_of(const void* p, int64_t ld, int rows, int cols, char** ws, Rows* out, hipStream_t s) {
-  if (!packed(p, ld, cols)) {
-    *out = {static_cast<const uint16_t*>(p), ld, cols};
-    return GD_OK;
-  }
-  const int per_row = pad8(cols) / 8;
-  const int64_t blocks = div_up(int64_t(rows) * per_row, 256);
-  GD_REQUIRE(blocks < (int64_t(1) << 31), "linear: grid too large");
-  uint16_t* dst = reinterpret_cast<uint16_t*>(*ws);
-  *ws += align256(size_t(rows) * per_row * 16);
-  if (rows > 0) {
-    hipLaunchKernelGGL(linear_pack, dim3(unsigned(blocks)), dim3(256), 0, s, static_cast<const uint16_t*>(p), ld, rows,
-                       cols, dst, per_row);
-    GD_LAUNCH_CHECK("linear_pack");
-  }
-  *out = {dst, pad8(cols), pad8(cols)};
-  return GD_OK;
-}
-size_t rows_bytes(bool pack, int rows, int cols) { return pack ? align256(size_t(rows) * pad8(cols) * 2) : 0; }
+Rows rows_of(const void* p, int64_t ld, int cols) { return {static_cast<const uint16_t*>(p), ld, pad8(cols)}; }
 
 Epi plain_epi(void* y, bool f32, int64_t ldy) {
   Epi e = {};
@@ -847,9 +958,7 @@ template <typename E>
 gd_status forward(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int act, const void* res,
                   int res_dtype, int64_t ldr, int M, int K, int N, void* y, int y_dtype, int64_t ldy, void* z,
                   int64_t ldz, char* ws, hipStream_t s) {
-  Rows rx, rw;
-  GD_TRY(rows_of(x, ldx, M, K, &ws, &rx, s));
-  GD_TRY(rows_of(w, ldw, N, K, &ws, &rw, s));
+  const Rows rx = rows_of(x, ldx, K), rw = rows_of(w, ldw, K);
   Gemm g = {};
   g.a = rx.p;
   g.lda = rx.ld;
@@ -878,7 +987,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
                    int64_t lddx, void* dw, void* db, int param_dtype, char* ws, hipStream_t s) {
   const int n8 = pad8(N);
   Rows rz = {static_cast<const uint16_t*>(dy), lddy, N};
-  const bool make = act != kNone || dy_dtype == GD_F32 || packed(dy, lddy, N);
+  const bool make = act != kNone || dy_dtype == GD_F32 || !readable(dy, lddy, N, false);
   if (make && (dx || dw)) {
     rz = {reinterpret_cast<uint16_t*>(ws), n8, n8};
     ws += align256(size_t(M) * n8 * 2);
@@ -913,8 +1022,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     }
   }
   if (dx) {
-    Rows rw;
-    GD_TRY(rows_of(w, ldw, N, K, &ws, &rw, s));
+    const Rows rw = rows_of(w, ldw, K);
     Gemm g = {};
     g.a = rz.p;
     g.lda = rz.ld;
@@ -931,8 +1039,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     ws += p.bytes;
   }
   if (dw) {
-    Rows rx;
-    GD_TRY(rows_of(x, ldx, M, K, &ws, &rx, s));
+    const Rows rx = rows_of(x, ldx, K);
     Gemm g = {};
     g.a = rz.p;
     g.lda = rz.ld;
@@ -949,16 +1056,12 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
   return GD_OK;
 }
 
-size_t forward_bytes(bool pack_x, bool pack_w, int M, int K, int N) {
-  return rows_bytes(pack_x, M, K) + rows_bytes(pack_w, N, K) + plan_of(M, N, pad8(K)).bytes;
-}
-
-size_t backward_bytes(int M, int K, int N, bool dx, bool dw, bool db, bool pack_x, bool pack_w) {
+size_t backward_bytes(int M, int K, int N, bool dx, bool dw, bool db) {
   const int n8 = pad8(N);
   size_t b = dx || dw ? align256(size_t(M) * n8 * 2) : 0;
   if (db) b += align256(size_t(dact_plan(M, N).blocks) * N * sizeof(float));
-  if (dx) b += rows_bytes(pack_w, N, K) + plan_of(M, K, n8).bytes;
-  if (dw) b += rows_bytes(pack_x, M, K) + plan_of(N, K, M).bytes;
+  if (dx) b += plan_of(M, K, n8).bytes;
+  if (dw) b += plan_of(N, K, M).bytes;
   return b;
 }
 
@@ -967,27 +1070,55 @@ size_t backward_bytes(int M, int K, int N, bool dx, bool dw, bool db, bool pack_
 
 using namespace gd;
 
-extern "C" size_t gd_linear_forward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
-                                                    int K, int N) {
-  if (M <= 0 || K <= 0 || N <= 0) return 0;
-  return forward_bytes(packed(x, ldx, K), packed(w, ldw, K), M, K, N);
+extern "C" int gd_linear_readable(const void* p, int64_t ld, int cols, int padded) {
+  return readable(p, ld, cols, padded != 0);
+}
+
+extern "C" gd_status gd_linear_pack(const void* a, int64_t lda, int rows_a, const void* b, int64_t ldb, int rows_b,
+                                    int cols, void* a_out, void* b_out, gd_stream_t stream) {
+  GD_REQUIRE(cols > 0 && cols <= kMaxPitch && rows_a >= 0 && rows_b >= 0 && rows_a <= (1 << 30) && rows_b <= (1 << 30),
+             "linear_pack: %d and %d rows of %d", rows_a, rows_b, cols);
+  GD_REQUIRE(rows_a == 0 || (a && a_out && aligned(a, 2) && aligned(a_out, 16) && lda >= cols), "linear_pack: first matrix");
+  GD_REQUIRE(rows_b == 0 || (b && b_out && aligned(b, 2) && aligned(b_out, 16) && ldb >= cols), "linear_pack: second matrix");
+  Pack p;
+  p.src[0] = static_cast<const uint16_t*>(a);
+  p.src[1] = static_cast<const uint16_t*>(b);
+  p.dst[0] = static_cast<uint16_t*>(a_out);
+  p.dst[1] = static_cast<uint16_t*>(b_out);
+  p.ld[0] = lda;
+  p.ld[1] = ldb;
+  p.cols = cols;
+  p.per_row = pad8(cols) / 8;
+  p.pieces[0] = int64_t(rows_a) * p.per_row;
+  p.pieces[1] = int64_t(rows_b) * p.per_row;
+  const int64_t blocks = div_up(p.pieces[0] + p.pieces[1], 256);
+  if (blocks == 0) return GD_OK;
+  GD_REQUIRE(blocks < (int64_t(1) << 31), "linear_pack: grid too large");
+  hipLaunchKernelGGL(linear_pack, dim3(unsigned(blocks)), dim3(256), 0, as_hip(stream), p);
+  GD_LAUNCH_CHECK("linear_pack");
+  return GD_OK;
+}
+
+extern "C" size_t gd_linear_forward_workspace_bytes(int M, int K, int N) {
+  return M > 0 && K > 0 && N > 0 ? plan_of(M, N, pad8(K)).bytes : 0;
 }
 
 extern "C" gd_status gd_linear_forward(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw,
                                        const void* bias, int act, const void* residual, int residual_dtype,
                                        int64_t ldr, int M, int K, int N, void* y, int y_dtype, int64_t ldy, void* z,
-                                       int64_t ldz, void* workspace, size_t workspace_bytes, gd_stream_t stream) {
+                                       int64_t ldz, int padded, void* workspace, size_t workspace_bytes, gd_stream_t stream) {
   GD_TRY(check_shape(dtype, act, M, K, N));
   if (M == 0) return GD_OK;
   GD_REQUIRE(x && w && y && ldx >= K && ldw >= K && ldy >= N, "linear: null pointer or short rows");
-  GD_REQUIRE(aligned(x, 2) && aligned(w, 2) && aligned(bias, 2), "linear: misaligned operands");
+  GD_REQUIRE(readable(x, ldx, K, padded) && readable(w, ldw, K, padded) && aligned(bias, 2),
+             "linear: x and W need rows of 16-byte pieces (gd_linear_pack)");
   GD_REQUIRE(!residual || (ldr >= N && (residual_dtype == dtype || residual_dtype == GD_F32)),
              "linear: the residual is fp32 or of the operands' type");
   GD_REQUIRE(y_dtype == (residual ? residual_dtype : dtype), "linear: y has the residual's type, without one x's");
   GD_REQUIRE(aligned(y, y_dtype == GD_F32 ? 4 : 2) && aligned(residual, residual_dtype == GD_F32 ? 4 : 2),
              "linear: misaligned y or residual");
   GD_REQUIRE(!z || (aligned(z, 16) && ldz % 8 == 0 && ldz >= pad8(N)), "linear: z has rows padded to 8 values");
-  const size_t want = forward_bytes(packed(x, ldx, K), packed(w, ldw, K), M, K, N);
+  const size_t want = plan_of(M, N, pad8(K)).bytes;
   GD_REQUIRE(workspace_bytes >= want && (want == 0 || (workspace && aligned(workspace, 16))),
              "linear: workspace of %zu bytes, %zu wanted", workspace_bytes, want);
   char* ws = static_cast<char*>(workspace);
@@ -998,16 +1129,14 @@ extern "C" gd_status gd_linear_forward(int dtype, const void* x, int64_t ldx, co
                                           ldy, z, ldz, ws, s);
 }
 
-extern "C" size_t gd_linear_backward_workspace_bytes(const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
-                                                     int K, int N, int dx, int dw, int db) {
-  if (M <= 0 || K <= 0 || N <= 0) return 0;
-  return backward_bytes(M, K, N, dx, dw, db, packed(x, ldx, K), packed(w, ldw, K));
+extern "C" size_t gd_linear_backward_workspace_bytes(int M, int K, int N, int dx, int dw, int db) {
+  return M > 0 && K > 0 && N > 0 ? backward_bytes(M, K, N, dx, dw, db) : 0;
 }
 
 extern "C" gd_status gd_linear_backward(int dtype, int act, const void* dy, int dy_dtype, int64_t lddy, const void* z,
                                         int64_t ldz, const void* x, int64_t ldx, const void* w, int64_t ldw, int M,
                                         int K, int N, void* dx, int dx_dtype, int64_t lddx, void* dw, void* db,
-                                        int param_dtype, void* workspace, size_t workspace_bytes,
+                                        int param_dtype, int padded, void* workspace, size_t workspace_bytes,
                                         gd_stream_t stream) {
   GD_TRY(check_shape(dtype, act, M, K, N));
   GD_REQUIRE(M > 0, "linear: gradients of no rows");
@@ -1016,11 +1145,12 @@ extern "C" gd_status gd_linear_backward(int dtype, int act, const void* dy, int 
   GD_REQUIRE((dx_dtype == dtype || dx_dtype == GD_F32) && (param_dtype == dtype || param_dtype == GD_F32),
              "linear: gradients are fp32 or of the operands' type");
   GD_REQUIRE(act == kNone || (z && ldz >= N), "linear: the activation's slope needs z");
-  GD_REQUIRE(aligned(dy, dy_dtype == GD_F32 ? 4 : 2) && aligned(z, 2) && aligned(x, 2) && aligned(w, 2) &&
-                 aligned(dx, dx_dtype == GD_F32 ? 4 : 2) && aligned(dw, param_dtype == GD_F32 ? 4 : 2) &&
+  GD_REQUIRE(aligned(dy, dy_dtype == GD_F32 ? 4 : 2) && aligned(z, 2) && aligned(dx, dx_dtype == GD_F32 ? 4 : 2) && aligned(dw, param_dtype == GD_F32 ? 4 : 2) &&
                  aligned(db, param_dtype == GD_F32 ? 4 : 2),
              "linear: misaligned operands");
-  const size_t want = backward_bytes(M, K, N, dx, dw, db, packed(x, ldx, K), packed(w, ldw, K));
+  GD_REQUIRE((!dw || readable(x, ldx, K, padded)) && (!dx || readable(w, ldw, K, padded)),
+             "linear: x and W need rows of 16-byte pieces (gd_linear_pack)");
+  const size_t want = backward_bytes(M, K, N, dx, dw, db);
   GD_REQUIRE(workspace_bytes >= want && (want == 0 || (workspace && aligned(workspace, 16))),
              "linear: workspace of %zu bytes, %zu wanted", workspace_bytes, want);
   GD_REQUIRE(dact_plan(M, N).slabs < 65536, "linear: N=%d", N);

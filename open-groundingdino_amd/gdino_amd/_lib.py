@@ -86,7 +86,8 @@ def lib() -> ctypes.CDLL:
 
 _host = None        # the C++ host side (gdino_amd._host) ...
 _host_bound = None  # ... and the library whose entry points it holds
-_HOST_ENTRY_POINTS = ("gd_last_error", "gd_linear_forward_workspace_bytes", "gd_linear_forward",
+_HOST_ENTRY_POINTS = ("gd_last_error", "gd_linear_readable", "gd_linear_pack",
+                      "gd_linear_forward_workspace_bytes", "gd_linear_forward",
                       "gd_linear_backward_workspace_bytes", "gd_linear_backward", "gd_adamw_step",
                       "gd_grad_norm_workspace_bytes", "gd_grad_norm")
 

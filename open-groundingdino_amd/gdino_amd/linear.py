@@ -24,10 +24,12 @@ import torch.nn.functional as F
 from . import _lib, castcache, kernels
 
 _p, _i, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_lib.register("gd_linear_readable", [_p, _i64, _i, _i])
+_lib.register("gd_linear_pack", [_p, _i64, _i, _p, _i64, _i, _i, _p, _p, _p])
 _lib.register("gd_linear_forward", [_i, _p, _i64, _p, _i64, _p, _i, _p, _i, _i64, _i, _i, _i, _p, _i, _i64, _p, _i64,
-                                    _p, _sz, _p])
+                                    _i, _p, _sz, _p])
 _lib.register("gd_linear_backward", [_i, _i, _p, _i, _i64, _p, _i64, _p, _i64, _p, _i64, _i, _i, _i, _p, _i, _i64, _p,
-                                     _p, _i, _p, _sz, _p])
+                                     _p, _i, _i, _p, _sz, _p])
 
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 DTYPES = (torch.bfloat16, torch.float16)

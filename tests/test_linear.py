@@ -32,12 +32,12 @@ def test_linear_act(emulated, m, k, n, act, dtype, residual, bias):
 
 
 @pytest.mark.parametrize("tile", ["64", "128", "256"])
-@pytest.mark.parametrize("m,k,n,act,dtype", [(150, 72, 136, "gelu", BF), (129, 200, 8, "none", HF),
-                                             (1100, 8, 24, "relu", BF), (3, 1030, 16, "silu", BF)])
-def test_tiles(emulated, monkeypatch, tile, m, k, n, act, dtype):
+@pytest.mark.parametrize("m,k,n,act,dtype,residual", [(150, 72, 136, "gelu", BF, F32), (129, 200, 8, "none", HF, HF),
+                                                      (1100, 8, 24, "relu", BF, None), (3, 1030, 16, "silu", BF, BF)])
+def test_tiles(emulated, monkeypatch, tile, m, k, n, act, dtype, residual):
     """Both tiles in every layout of the operands, with ragged edges and with sums over r that are split."""
     monkeypatch.setenv("GD_LINEAR_TILE", tile)
-    x, w, b, r, dy = lc.inputs(m, k, n, dtype, True, None, seed=2)
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, True, residual, seed=2)
     y, grads = lc.run(x, w, b, act, r, dy)
     lc.check(x, w, b, act, r, y, dy, grads)
 
@@ -152,15 +152,18 @@ def test_refusals(emulated):
     with pytest.raises(TypeError, match="residual"):
         linear_act(x, w, b, "none", r.half())
     y = torch.empty(6, 16, dtype=BF)
-    args = (2, x.data_ptr(), 24, w.data_ptr(), 24, None, 0, None, 2, 0, 6, 24, 16, y.data_ptr(), 2, 16, None, 0)
+    args = (2, x.data_ptr(), 24, w.data_ptr(), 24, None, 0, None, 2, 0, 6, 24, 16, y.data_ptr(), 2, 16, None, 0, 0)
     _lib.call("gd_linear_forward", *args, None, 0, None)
     for bad in ({0: 0}, {2: 8}, {6: 9}, {11: 0}, {13: None}, {14: 0}, {16: y.data_ptr() + 2, 17: 16}):
         call = [bad.get(i, a) for i, a in enumerate(args)]
         with pytest.raises(_lib.GdError):
             _lib.call("gd_linear_forward", *call, None, 0, None)
-    packed = [{2: 25}.get(i, a) for i, a in enumerate(args)]  # rows to pack, and no workspace
+    unreadable = [{2: 25}.get(i, a) for i, a in enumerate(args)]
+    with pytest.raises(_lib.GdError, match="gd_linear_pack"):
+        _lib.call("gd_linear_forward", *unreadable, None, 0, None)
+    split = [{11: 4096, 2: 4096, 4: 4096}.get(i, a) for i, a in enumerate(args)]  # (refused before it reads)
     with pytest.raises(_lib.GdError, match="workspace"):
-        _lib.call("gd_linear_forward", *packed, None, 0, None)
+        _lib.call("gd_linear_forward", *split, None, 0, None)
 
 
 def test_cpu_tensors_raise():

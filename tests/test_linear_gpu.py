@@ -120,7 +120,7 @@ def test_rows_behind_the_last_are_left():
     x, w, b, _, _ = lc.inputs(m, k, n, BF, device="cuda", grad=False)
     y = torch.full((m * n + 4096,), 7.0, dtype=BF, device="cuda")
     _lib.call("gd_linear_forward", 2, x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), 0, None, 2, 0, m, k, n,
-              y.data_ptr(), 2, n, None, 0, None, 0, _lib.stream_of(y))
+              y.data_ptr(), 2, n, None, 0, 0, None, 0, _lib.stream_of(y))
     assert (y[m * n:] == 7).all()
     lc.check(x, w, b, "none", None, y[:m * n].view(m, n))
 
