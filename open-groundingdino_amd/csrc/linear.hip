@@ -42,6 +42,10 @@ typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
                      "+a"((r)[6]), "+a"((r)[7]))
 #endif
 
+#ifndef GD_STORE_NT
+#define GD_STORE_NT(value, to) __builtin_nontemporal_store(value, to)
+#endif
+
 // the two 16-bit types
 struct Bf16 {
   static __device__ __forceinline__ float up(uint16_t h) { return bf16_to_f32(h); }
@@ -183,6 +187,24 @@ __device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool ve
   for (int j = 0; j < 8; ++j) v[j] = E::up(w.h[j]);
 }
 
+// 16 bytes of an output, which nothing reads soon: past the caches' ways of lines that are kept
+// (16384 x 512 -> 4096: 112 us with plain stores, 102 with these; 44446 x 256 -> 2048: 108 and 98)
+__device__ __forceinline__ void st_out(uint16_t* p, uint4 u) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  GD_STORE_NT((u32x4{u.x, u.y, u.z, u.w}), reinterpret_cast<u32x4*>(p));
+}
+
+template <typename E>
+__device__ __forceinline__ uint4 pack8(const float v[8]) {
+  union {
+    uint4 u;
+    uint16_t h[8];
+  } w;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
+  return w.u;
+}
+
 template <typename E>
 __device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int left, const float v[8]) {
   if (f32) {
@@ -205,7 +227,7 @@ __device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int
 #pragma unroll
   for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
   if (vec && left >= 8) {
-    *reinterpret_cast<uint4*>(q) = w.u;
+    st_out(q, w.u);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -263,8 +285,8 @@ constexpr int kR = 64;  // values of r per staged chunk
 struct Tile {
   int m, n, split;
 };
-__device__ __forceinline__ Tile tile_of(const Gemm& p) {
-  const int L = xcd_remap(int(blockIdx.x), int(gridDim.x));
+__device__ __forceinline__ Tile tile_of(const Gemm& p, int block, int blocks) {
+  const int L = xcd_remap(block, blocks);
   const int tiles = p.tiles_m * p.tiles_n;
   Tile t;
   t.split = L / tiles;
@@ -311,7 +333,8 @@ __device__ __forceinline__ gd_i16x8 fragment(const uint16_t* img, int x0, int s,
 // of 16 bytes to consecutive LDS positions, so the swizzle is applied to the source: position pos of a row holds
 // its chunk pos ^ swz.  Rows (columns) past the operand's end read its last one instead: their products land in
 // outputs that are not stored.
-template <int X, bool COL, int WAVES>
+// PAIRS: of 32 rows, those whose products one lane of two blocks holds (4 each) follow each other.
+template <int X, bool COL, int WAVES, bool PAIRS = false>
 struct Loader {
   static constexpr int kInstr = X * 8 / 64 / WAVES;  // per wave and chunk
   static_assert(kInstr * 64 * WAVES == X * 8, "the waves share an image evenly");
@@ -328,7 +351,9 @@ struct Loader {
         const int r = piece / (X / 8), x = 8 * ((piece % (X / 8)) ^ col_swz<X>(r));
         offset[h] = uint32_t(r * uint32_t(ld) + (x0 + x < cols ? x : cols - 8 - x0)) * 2;
       } else {
-        const int row = piece >> 3, x = x0 + row < end ? row : end - 1 - x0;
+        const int row = piece >> 3;
+        const int from = PAIRS ? (row & ~31) + 8 * ((row >> 2) & 3) + 4 * ((row >> 4) & 1) + (row & 3) : row;
+        const int x = x0 + from < end ? from : end - 1 - x0;
         offset[h] = (uint32_t(x) * uint32_t(ld) + 8 * ((piece & 7) ^ row_swz(row))) * 2;
       }
     }
@@ -520,7 +545,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[ST * kStage];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / WN, wn = wave % WN;
-  const Tile t = tile_of(p);
+  const Tile t = tile_of(p, int(blockIdx.x), int(gridDim.x));
   const int m0 = t.m * BM, n0 = t.n * BN, split = t.split;
   const int r_end = p.ra > p.rb ? p.ra : p.rb, r_both = p.ra < p.rb ? p.ra : p.rb;
   const int rb0 = split * p.r_per_split;
@@ -602,7 +627,7 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[kRing * kImg];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave >> 1, wn = wave & 1;
-  const Tile t = tile_of(p);
+  const Tile t = tile_of(p, int(blockIdx.x), int(gridDim.x));
   const int m0 = t.m * BX, n0 = t.n * BX, split = t.split;
   const int r_end = p.ra > p.rb ? p.ra : p.rb, r_both = p.ra < p.rb ? p.ra : p.rb;
   const int rb0 = split * p.r_per_split;
@@ -697,6 +722,165 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   for (int i = 1; i < T; ++i) GD_MMA_WAIT8("", acc[i]);
   store_tile<E, T, T, 4, !AC && !BC>(p, acc, reinterpret_cast<float*>(lds) + wave * kOwn, m0 + 16 * wm * T,
                                      n0 + 16 * wn * T, split, lane);
+}
+
+// 128 x 128 tiles of a layer with few features in, by workgroups that go from tile to tile: the next tile's first two
+// chunks are asked for before the output is stored, straight from the registers (a lane holds 8 consecutive
+// columns of a row), so loads, products and stores of the two workgroups of a CU run side by side.  For whole pieces
+// only (see `streams`).
+template <typename E>
+__global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
+  constexpr int T = 4, kWaves = 4, BX = 128, kStage = 2 * BX * kR;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStage];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave >> 1, wn = wave & 1, c = lane & 15, g = lane >> 4;
+  const int chunks = p.ra / kR, tiles = p.tiles_m * p.tiles_n;
+  using LA = Loader<BX, false, kWaves>;
+  using LB = Loader<BX, false, kWaves, true>;
+  constexpr int kInstr = LA::kInstr + LB::kInstr, kStores = 2 * T;  // of a wave: per chunk; per tile at least
+  Tile t = tile_of(p, int(blockIdx.x), tiles);
+  LA la(p.a, p.lda, t.m * BX, p.M, p.ca, 0, wave, lane);
+  LB lb(p.b, p.ldb, t.n * BX, p.N, p.cb, 0, wave, lane);
+  uint32_t now = 0;  // the image of the chunk at hand
+  auto issue = [&](uint32_t image) {
+    la.issue(lds, image * (2 * kStage), wave);
+    lb.issue(lds, image * (2 * kStage) + 2 * BX * kR, wave);
+  };
+  // the bias of a lane's 2 x 8 columns
+  auto bias_of = [&](int n0, uint4 (&b)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int n = n0 + 64 * wn + 32 * h + 8 * g;
+      b[h] = p.epi.bias ? *reinterpret_cast<const uint4*>(p.epi.bias + (n < p.N ? n : p.N - 8)) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  uint4 braw[2];
+  issue(0);
+  bias_of(t.n * BX, braw);
+  issue(1);
+  bool stored = false;  // at least kStores stores of this wave follow the chunks under way
+  for (int v = int(blockIdx.x); v < tiles; v += int(gridDim.x)) {
+    const int m0 = t.m * BX + 64 * wm, n0 = t.n * BX + 64 * wn;
+    const bool whole = t.m * BX + BX <= p.M && t.n * BX + BX <= p.N;
+    const bool more = v + int(gridDim.x) < tiles;
+    gd_f32x4 acc[T][T];
+#pragma unroll
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < T; ++j) acc[i][j] = gd_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < chunks; ++k) {
+      if (k == 0) {
+        if (stored)
+          gd_wait_vmcnt(kInstr + kStores);
+        else
+          gd_wait_vmcnt(kInstr);
+      } else if (k == 1 && stored) {
+        gd_wait_vmcnt(kStores);
+      } else {
+        gd_wait_vmcnt(0);
+      }
+      gd_lds_barrier();
+      if (k + 1 == chunks) {
+        if (more) {
+          t = tile_of(p, v + int(gridDim.x), tiles);
+          la = LA(p.a, p.lda, t.m * BX, p.M, p.ca, 0, wave, lane);
+          lb = LB(p.b, p.ldb, t.n * BX, p.N, p.cb, 0, wave, lane);
+          issue(now ^ 1);
+        }
+      } else if (k > 0) {
+        issue(now ^ 1);
+      }
+      const uint16_t* const img = lds + now * kStage;
+#pragma unroll
+      for (int s = 0; s < kR / 32; ++s) {
+        gd_i16x8 fa[T], fb[T];
+#pragma unroll
+        for (int j = 0; j < T; ++j) fb[j] = fragment<BX, false>(img + BX * kR, 16 * (wn * T + j), s, lane);
+#pragma unroll
+        for (int i = 0; i < T; ++i) fa[i] = fragment<BX, false>(img, 16 * (wm * T + i), s, lane);
+#pragma unroll
+        for (int i = 0; i < T; ++i)
+#pragma unroll
+          for (int j = 0; j < T; ++j) acc[i][j] = E::mma(fb[j], fa[i], acc[i][j]);
+      }
+      now ^= 1;
+    }
+    union {
+      uint4 u[2];
+      uint16_t h[16];
+    } bias;
+    bias.u[0] = braw[0];
+    bias.u[1] = braw[1];
+    uint4 res[2 * T][2];
+    if (p.epi.res) {
+      const char* const from = static_cast<const char*>(p.epi.res);
+      const int64_t size = p.epi.res_f32 ? 4 : 2;
+#pragma unroll
+      for (int q = 0; q < 2 * T; ++q) {
+        const int m = m0 + 16 * (q >> 1) + c, n = n0 + 32 * (q & 1) + 8 * g;
+        const uint4* const r = reinterpret_cast<const uint4*>(
+            from + ((m < p.M ? m : p.M - 1) * p.epi.ldr + (n < p.N ? n : p.N - 8)) * size);
+        res[q][0] = r[0];
+        res[q][1] = r[p.epi.res_f32 ? 1 : 0];
+      }
+    }
+    gd_lds_barrier();  // the last chunk has been read
+    if (more) {
+      bias_of(t.n * BX, braw);
+      issue(now ^ 1);
+    }
+    const bool odd = (lane & 1) != 0;
+    // pieces of row c, columns 8 g and 32 + 8 g: lanes c and c ^ 1 trade one, so that an instruction writes whole rows of
+    // 128 bytes (64 bytes of twice the rows take twice the time)
+    auto write = [&](uint16_t* to, int64_t ld, int i, uint4 first, uint4 second) {
+      const uint4 give = odd ? first : second;
+      uint4 take;
+      take.x = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.x)));
+      take.y = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.y)));
+      take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
+      take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
+      const int m = m0 + 16 * i + (c & 14), n = n0 + 8 * g + (odd ? 32 : 0);
+      uint16_t* const at = to + m * ld + n;
+      if (m < p.M && n < p.N) st_out(at, odd ? take : first);
+      if (m + 1 < p.M && n < p.N) st_out(at + ld, odd ? second : take);
+    };
+    auto store = [&](auto ACT) {
+#pragma unroll
+      for (int i = 0; i < T; ++i) {
+        uint4 y[2], z[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = acc[i][2 * h + (j >> 2)][j & 3] + E::up(bias.h[8 * h + j]);
+          if (p.epi.z) z[h] = pack8<E>(x);
+          activate8(x, decltype(ACT)::value);
+          if (p.epi.res) {
+            union {
+              uint4 u[2];
+              uint16_t h16[8];
+              float f[8];
+            } raw;
+            raw.u[0] = res[2 * i + h][0];
+            raw.u[1] = res[2 * i + h][1];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] += p.epi.res_f32 ? raw.f[j] : E::up(raw.h16[j]);
+          }
+          y[h] = pack8<E>(x);
+        }
+        if (p.epi.z) write(p.epi.z, p.epi.ldz, i, z[0], z[1]);
+        write(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, i, y[0], y[1]);
+      }
+    };
+    switch (p.epi.act) {
+      case kRelu: store(std::integral_constant<int, kRelu>()); break;
+      case kGelu: store(std::integral_constant<int, kGelu>()); break;
+      case kGeluTanh: store(std::integral_constant<int, kGeluTanh>()); break;
+      case kSilu: store(std::integral_constant<int, kSilu>()); break;
+      default: store(std::integral_constant<int, kNone>()); break;
+    }
+    stored = whole;
+  }
 }
 
 // the parts added in order, then the epilogue; a thread per 8 columns
@@ -878,6 +1062,12 @@ Plan plan_of(int M, int N, int r) {
   return p;
 }
 
+// whether linear_stream takes a layer: whole chunks, at least two, and whole aligned pieces in every row
+bool streams(const Gemm& g) {
+  return g.ra == g.rb && g.ra % kR == 0 && g.ra >= 2 * kR && g.N % 8 == 0 && !g.epi.y_f32 && g.epi.y_vec &&
+         (!g.epi.bias || g.epi.bias_vec) && (!g.epi.res || g.epi.res_vec);
+}
+
 template <typename E, bool AC, bool BC>
 gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.splits = plan.splits;
@@ -888,7 +1078,10 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.group = plan.tile == 256 ? 4 : 8;  // (32 or 64 workgroups per XCD at a time)
   const int64_t grid = int64_t(g.tiles_m) * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
-  if (plan.tile == 256)
+  if (!AC && !BC && plan.tile == 128 && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g)) {
+    const int64_t at_once = env_int("GD_LINEAR_GROUPS", 512);
+    hipLaunchKernelGGL(linear_stream<E>, dim3(unsigned(grid < at_once ? grid : at_once)), dim3(256), 0, s, g);
+  } else if (plan.tile == 256)
     hipLaunchKernelGGL((linear_gemm256<E, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   else if (plan.tile == 128)
     hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);

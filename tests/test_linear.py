@@ -42,6 +42,18 @@ def test_tiles(emulated, monkeypatch, tile, m, k, n, act, dtype, residual):
     lc.check(x, w, b, act, r, y, dy, grads)
 
 
+@pytest.mark.parametrize("groups", ["1", "3"])
+@pytest.mark.parametrize("m,k,n,act,dtype,residual", [(300, 128, 264, "gelu", BF, F32), (257, 192, 136, "relu", HF, None),
+                                                      (129, 256, 384, "silu", BF, BF), (520, 128, 8, "none", BF, BF)])
+def test_workgroups_over_many_tiles(emulated, monkeypatch, groups, m, k, n, act, dtype, residual):
+    """Few features in: a workgroup goes from tile to tile, whole ones and ragged ones, an odd and an even number of chunks."""
+    monkeypatch.setenv("GD_LINEAR_TILE", "128")
+    monkeypatch.setenv("GD_LINEAR_GROUPS", groups)
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, act != "silu", residual, seed=5)
+    y, grads = lc.run(x, w, b, act, r, dy)
+    lc.check(x, w, b, act, r, y, dy, grads)
+
+
 def test_strides_and_shapes(emulated):
     """Leading dimensions, transposed and sliced inputs, an expanded residual and gradient, a misaligned view."""
     from gdino_amd.linear import linear_act

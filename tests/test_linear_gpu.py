@@ -39,6 +39,17 @@ def test_tiles(monkeypatch, tile, m, k, n):
         lc.check(x, w, b, "gelu", r, y, dy, grads)
 
 
+@pytest.mark.parametrize("groups", ["8", "24", "512"])
+@pytest.mark.parametrize("m,k,n", [(1000, 128, 264), (2049, 192, 1032), (700, 256, 512), (3000, 512, 1024)])
+def test_workgroups_over_many_tiles(monkeypatch, groups, m, k, n):
+    monkeypatch.setenv("GD_LINEAR_TILE", "128")
+    monkeypatch.setenv("GD_LINEAR_GROUPS", groups)
+    for dtype, act, residual in ((BF, "relu", None), (HF, "gelu_tanh", HF), (BF, "silu", F32), (BF, "none", BF)):
+        x, w, b, r, dy = lc.inputs(m, k, n, dtype, act != "silu", residual, seed=k, device="cuda")
+        y, grads = lc.run(x, w, b, act, r, dy)
+        lc.check(x, w, b, act, r, y, dy, grads)
+
+
 def test_large_values():
     """Activations far from zero: nothing overflows on the way to a finite result."""
     from gdino_amd.linear import linear_act
