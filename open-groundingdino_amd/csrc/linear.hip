@@ -316,13 +316,15 @@ __device__ __forceinline__ gd_i16x4 lds_tr(const uint16_t* p) {
 }
 
 // the operand of one 16 x 16 x 32 product: lane (c, g) holds r = 8 g .. 8 g + 7 of row x0 + c, chunk s of 32
-template <int X, bool COL>
+// PAIRS: as Loader's, here for columns: of the two blocks of 32 columns, the one of x0 takes 4 of every 8
+template <int X, bool COL, bool PAIRS = false>
 __device__ __forceinline__ gd_i16x8 fragment(const uint16_t* img, int x0, int s, int lane) {
   if constexpr (!COL) {
     return *reinterpret_cast<const gd_i16x8*>(img + row_at(x0 + (lane & 15), 4 * s + (lane >> 4)));
   } else {
     const int g = lane >> 4, q = (lane >> 2) & 3, p = lane & 3;
-    const int ch = (x0 >> 3) + (p >> 1), sub = 4 * (p & 1);
+    const int ch = PAIRS ? ((x0 >> 3) & ~3) + p : (x0 >> 3) + (p >> 1);
+    const int sub = 4 * (PAIRS ? (x0 >> 4) & 1 : p & 1);
     const gd_i16x4 lo = lds_tr(img + col_at<X>(32 * s + 8 * g + q, ch) + sub);
     const gd_i16x4 hi = lds_tr(img + col_at<X>(32 * s + 8 * g + 4 + q, ch) + sub);
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -728,7 +730,7 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
 // chunks are asked for before the output is stored, straight from the registers (a lane holds 8 consecutive
 // columns of a row), so loads, products and stores of the two workgroups of a CU run side by side.  For whole pieces
 // only (see `streams`).
-template <typename E>
+template <typename E, bool BC>
 __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
   constexpr int T = 4, kWaves = 4, BX = 128, kStage = 2 * BX * kR;
   __shared__ __attribute__((aligned(16))) uint16_t lds[2 * kStage];
@@ -736,7 +738,7 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
   const int wm = wave >> 1, wn = wave & 1, c = lane & 15, g = lane >> 4;
   const int chunks = p.ra / kR, tiles = p.tiles_m * p.tiles_n;
   using LA = Loader<BX, false, kWaves>;
-  using LB = Loader<BX, false, kWaves, true>;
+  using LB = Loader<BX, BC, kWaves, !BC>;
   constexpr int kInstr = LA::kInstr + LB::kInstr, kStores = 2 * T;  // of a wave: per chunk; per tile at least
   Tile t = tile_of(p, int(blockIdx.x), tiles);
   LA la(p.a, p.lda, t.m * BX, p.M, p.ca, 0, wave, lane);
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
       for (int s = 0; s < kR / 32; ++s) {
         gd_i16x8 fa[T], fb[T];
 #pragma unroll
-        for (int j = 0; j < T; ++j) fb[j] = fragment<BX, false>(img + BX * kR, 16 * (wn * T + j), s, lane);
+        for (int j = 0; j < T; ++j) fb[j] = fragment<BX, BC, BC>(img + BX * kR, 16 * (wn * T + j), s, lane);
 #pragma unroll
         for (int i = 0; i < T; ++i) fa[i] = fragment<BX, false>(img, 16 * (wm * T + i), s, lane);
 #pragma unroll
@@ -1078,9 +1080,9 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   g.group = plan.tile == 256 ? 4 : 8;  // (32 or 64 workgroups per XCD at a time)
   const int64_t grid = int64_t(g.tiles_m) * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
-  if (!AC && !BC && plan.tile == 128 && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g)) {
+  if (!AC && plan.tile == 128 && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g)) {
     const int64_t at_once = env_int("GD_LINEAR_GROUPS", 512);
-    hipLaunchKernelGGL(linear_stream<E>, dim3(unsigned(grid < at_once ? grid : at_once)), dim3(256), 0, s, g);
+    hipLaunchKernelGGL((linear_stream<E, BC>), dim3(unsigned(grid < at_once ? grid : at_once)), dim3(256), 0, s, g);
   } else if (plan.tile == 256)
     hipLaunchKernelGGL((linear_gemm256<E, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   else if (plan.tile == 128)
