@@ -205,7 +205,7 @@ __device__ __forceinline__ uint4 pack8(const float v[8]) {
   return w.u;
 }
 
-template <typename E>
+template <typename E, bool NT = true>
 __device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int left, const float v[8]) {
   if (f32) {
     float* q = static_cast<float*>(p) + at;
@@ -227,7 +227,10 @@ __device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int
 #pragma unroll
   for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
   if (vec && left >= 8) {
-    st_out(q, w.u);
+    if (NT)
+      st_out(q, w.u);
+    else
+      *reinterpret_cast<uint4*>(q) = w.u;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
@@ -726,6 +729,25 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
                                      n0 + 16 * wn * T, split, lane);
 }
 
+// 16 rows of 64 columns from m, n on: lane (c, g) has the pieces of row c, columns 8 g and 32 + 8 g.  Lanes c and c ^ 1 trade
+// one, so that an instruction writes whole rows of 128 bytes (64 bytes of twice the rows take twice the time:
+// 199 us against 82 for 44446 x 256 -> 2048).
+__device__ __forceinline__ void write_rows(uint16_t* to, int64_t ld, int m, int n, int M, int N, int lane, uint4 first,
+                                           uint4 second) {
+  const bool odd = (lane & 1) != 0;
+  const uint4 give = odd ? first : second;
+  uint4 take;
+  take.x = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.x)));
+  take.y = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.y)));
+  take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
+  take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
+  m += lane & 14;
+  n += 8 * (lane >> 4) + (odd ? 32 : 0);
+  uint16_t* const at = to + m * ld + n;
+  if (m < M && n < N) st_out(at, odd ? take : first);
+  if (m + 1 < M && n < N) st_out(at + ld, odd ? second : take);
+}
+
 // 128 x 128 tiles of a layer with few features in, by workgroups that go from tile to tile: the next tile's first two
 // chunks are asked for before the output is stored, straight from the registers (a lane holds 8 consecutive
 // columns of a row), so loads, products and stores of the two workgroups of a CU run side by side.  For whole pieces
@@ -831,21 +853,6 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
       bias_of(t.n * BX, braw);
       issue(now ^ 1);
     }
-    const bool odd = (lane & 1) != 0;
-    // pieces of row c, columns 8 g and 32 + 8 g: lanes c and c ^ 1 trade one, so that an instruction writes whole rows of
-    // 128 bytes (64 bytes of twice the rows take twice the time)
-    auto write = [&](uint16_t* to, int64_t ld, int i, uint4 first, uint4 second) {
-      const uint4 give = odd ? first : second;
-      uint4 take;
-      take.x = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.x)));
-      take.y = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.y)));
-      take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
-      take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
-      const int m = m0 + 16 * i + (c & 14), n = n0 + 8 * g + (odd ? 32 : 0);
-      uint16_t* const at = to + m * ld + n;
-      if (m < p.M && n < p.N) st_out(at, odd ? take : first);
-      if (m + 1 < p.M && n < p.N) st_out(at + ld, odd ? second : take);
-    };
     auto store = [&](auto ACT) {
 #pragma unroll
       for (int i = 0; i < T; ++i) {
@@ -870,8 +877,8 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
           }
           y[h] = pack8<E>(x);
         }
-        if (p.epi.z) write(p.epi.z, p.epi.ldz, i, z[0], z[1]);
-        write(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, i, y[0], y[1]);
+        if (p.epi.z) write_rows(p.epi.z, p.epi.ldz, m0 + 16 * i, n0, p.M, p.N, lane, z[0], z[1]);
+        write_rows(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, m0 + 16 * i, n0, p.M, p.N, lane, y[0], y[1]);
       }
     };
     switch (p.epi.act) {
@@ -945,7 +952,7 @@ __global__ void __launch_bounds__(256) linear_dact(const Dact p) {
         const int64_t row = m + h * rows;
         if (row < end) {
           if (p.z) slope8(d[h], z[h], p.act);  // (beyond `left` both are zero)
-          if (p.dz) st8<E>(p.dz, row * p.lddz + n, false, true, 8, d[h]);
+          if (p.dz) st8<E, false>(p.dz, row * p.lddz + n, false, true, 8, d[h]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) sum[j] += d[h][j];
         }
@@ -966,21 +973,169 @@ __global__ void __launch_bounds__(256) linear_dact(const Dact p) {
 }
 
 // db[n] = sum of `parts` rows; 32 columns and 8 groups of rows per workgroup, the groups' sums added in order
+// dz = dy * act'(z) and dx = dz W together, for layers with up to 256 features in: a workgroup's tile of dx has all of
+// its columns, so dy and z are read once, and dz is not read back for dx (it is written where dW needs it).  A
+// chunk's dy and z are asked for a chunk ahead, into registers; their dz goes to LDS as the product's operand A, while
+// W's chunk comes by LDS-DMA.  64 rows by 64 WN columns: small, so that three workgroups of a CU wait for memory in turn
+// (128 rows need more registers than two workgroups of a CU have: 349 us against 125 for 44446 x 256 <- 2048, which
+// moves 570 MB; apart the two take 190, since dz's way out goes on while it is read back).
+constexpr int kSumThreads = 1024;
+struct DzDx {
+  const uint16_t *dy, *z, *w;
+  uint16_t *dz, *dx;  // dz: or NULL
+  float* sums;        // or NULL: [workgroups][N]
+  int64_t lddy, ldz, lddz, ldw, lddx;
+  int M, K, N, act, w_cols;
+};
+
+constexpr int kTogetherRows = 64;
+template <typename E, int WN>
+__global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
+  constexpr int kWaves = 4, BM = kTogetherRows, BN = 64 * WN, TM = BM / 16 * WN / kWaves, TN = 4;
+  constexpr int kA = BM * kR, kB = BN * kR, kPieces = BM * kR / 8 / 256;
+  __shared__ __attribute__((aligned(16))) uint16_t lds[kA + kB];
+  __shared__ float4 lds_sums[kWaves][kR / 4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / WN, wn = wave % WN;
+  const int m0 = int(blockIdx.x) * BM, chunks = p.N / kR;
+  const int row = int(threadIdx.x >> 3), ch = int(threadIdx.x & 7);  // of a thread's first piece, 32 rows to the next
+  Loader<BN, true, kWaves> lw(p.w, p.ldw, 0, p.K, p.w_cols, 0, wave, lane);
+  // (rows past the end are the last one again, and count as zero)
+  const char* dy = reinterpret_cast<const char*>(p.dy + int64_t(m0) * p.lddy);
+  const char* z = reinterpret_cast<const char*>(p.z + int64_t(m0) * p.ldz);
+  uint32_t dy_at[kPieces], z_at[kPieces];  // bytes (the host keeps row pitches below kMaxPitch)
+#pragma unroll
+  for (int h = 0; h < kPieces; ++h) {
+    const int r = m0 + row + 32 * h < p.M ? row + 32 * h : p.M - 1 - m0;
+    dy_at[h] = (uint32_t(r) * uint32_t(p.lddy) + 8 * ch) * 2;
+    z_at[h] = (uint32_t(r) * uint32_t(p.ldz) + 8 * ch) * 2;
+  }
+  uint16_t* dz = p.dz + int64_t(m0 + row) * p.lddz + 8 * ch;
+  uint4 dy_of[kPieces], z_of[kPieces];
+  auto ask = [&]() {
+#pragma unroll
+    for (int h = 0; h < kPieces; ++h) {
+      dy_of[h] = *reinterpret_cast<const uint4*>(dy + dy_at[h]);
+      z_of[h] = *reinterpret_cast<const uint4*>(z + z_at[h]);
+    }
+    dy += 2 * kR;
+    z += 2 * kR;
+  };
+  gd_f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = gd_f32x4{0.f, 0.f, 0.f, 0.f};
+  ask();
+  for (int k = 0; k < chunks; ++k) {
+    if (k > 0) gd_lds_barrier();  // the last chunk's operands have been read
+    lw.issue(lds, 2 * kA, wave);
+    float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    auto slopes = [&](auto ACT) {
+#pragma unroll
+      for (int h = 0; h < kPieces; ++h) {
+        union {
+          uint4 u;
+          uint16_t h16[8];
+        } a, b;
+        a.u = dy_of[h];
+        b.u = z_of[h];
+        const bool in = m0 + row + 32 * h < p.M;
+        float d[8], zz[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          d[j] = E::up(a.h16[j]);
+          zz[j] = E::up(b.h16[j]);
+        }
+        slope8(d, zz, decltype(ACT)::value);
+        const uint4 u = pack8<E>(d);
+        *reinterpret_cast<uint4*>(lds + row_at(row + 32 * h, ch)) = u;
+        if (in) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[j] += d[j];
+          if (p.dz) *reinterpret_cast<uint4*>(dz + 32 * h * p.lddz) = u;
+        }
+      }
+    };
+    switch (p.act) {
+      case kRelu: slopes(std::integral_constant<int, kRelu>()); break;
+      case kGelu: slopes(std::integral_constant<int, kGelu>()); break;
+      case kGeluTanh: slopes(std::integral_constant<int, kGeluTanh>()); break;
+      default: slopes(std::integral_constant<int, kSilu>()); break;
+    }
+    dz += kR;
+    if (p.sums) {  // over the wave's 8 rows of lanes
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum[j] += dpp<DPP_ROR8>(sum[j]);
+        sum[j] += __shfl_xor(sum[j], 16, 64);
+        sum[j] += __shfl_xor(sum[j], 32, 64);
+      }
+      if (lane < 8) {
+        lds_sums[wave][2 * ch] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        lds_sums[wave][2 * ch + 1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+      }
+    }
+    // W's chunk has landed: it is older than dz's stores (in a tile with all its rows every wave has them) and the next
+    // chunk of dy and z
+    if (k + 1 < chunks) {
+      ask();
+      if (p.dz && m0 + BM <= p.M)
+        gd_wait_vmcnt(3 * kPieces);
+      else
+        gd_wait_vmcnt(2 * kPieces);
+    } else {
+      gd_wait_vmcnt(0);
+    }
+    gd_lds_barrier();
+    if (p.sums && threadIdx.x < kR) {
+      const float* const s = reinterpret_cast<const float*>(lds_sums) + threadIdx.x;
+      p.sums[int64_t(blockIdx.x) * p.N + k * kR + threadIdx.x] = (s[0] + s[kR]) + (s[2 * kR] + s[3 * kR]);
+    }
+    const uint16_t* const img = lds + kA;
+#pragma unroll
+    for (int s = 0; s < kR / 32; ++s) {
+      gd_i16x8 fa[TM];
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = fragment<BM, false>(lds, 16 * (wm * TM + i), s, lane);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const gd_i16x8 fb = fragment<BN, true, true>(img, 16 * (wn * TN + j), s, lane);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) acc[i][j] = E::mma(fb, fa[i], acc[i][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    uint4 x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
+      x[h] = pack8<E>(v);
+    }
+    write_rows(p.dx, p.lddx, m0 + 16 * (wm * TM + i), 64 * wn, p.M, p.K, lane, x[0], x[1]);
+  }
+}
+
 template <typename E>
-__global__ void __launch_bounds__(256) linear_colsum(const float* __restrict__ sums, int parts, int N,
+__global__ void __launch_bounds__(kSumThreads) linear_colsum(const float* __restrict__ sums, int parts, int N,
                                                      void* __restrict__ db, int f32) {
-  __shared__ float lds[8][32];
+  constexpr int kGroups = kSumThreads / 32;
+  __shared__ float lds[kGroups][32];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int n = int(blockIdx.x) * 32 + c;
   float s = 0.f;
   if (n < N) {
 #pragma unroll 8
-    for (int k = g; k < parts; k += 8) s += sums[int64_t(k) * N + n];
+    for (int k = g; k < parts; k += kGroups) s += sums[int64_t(k) * N + n];
   }
   lds[g][c] = s;
   __syncthreads();
   if (g == 0 && n < N) {
-    for (int k = 1; k < 8; ++k) s += lds[k][c];
+    for (int k = 1; k < kGroups; ++k) s += lds[k][c];
     if (f32)
       static_cast<float*>(db)[n] = s;
     else
@@ -1134,6 +1289,15 @@ DactPlan dact_plan(int M, int N) {
   return d;
 }
 
+// Whether the backward of an activation and dx are one kernel (the rest of the conditions is about the pieces).  Its
+// workgroups take some 1.8 us per chunk whatever their number, so it pays for many rows, and where dz on its way
+// through memory costs more than its place in the caches: 44446 x 256 <- 2048 218 us and 261 apart (the whole
+// backward), 33400 x 192 <- 768 81 and 91; 16384 x 256 <- 1024 66 and 62, 8192 x 256 <- 2048 79 and 58.
+bool dz_dx_fits(int M, int K, int N) {
+  const int from = env_int("GD_LINEAR_TOGETHER", 0);  // (A/B: rows)
+  return K <= 256 && (from > 0 ? M >= from : M >= 24576 && int64_t(M) * N >= 20000000);
+}
+
 #define GD_TRY(expr)                     \
   do {                                   \
     const gd_status _s = (expr);         \
@@ -1187,7 +1351,43 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     rz = {reinterpret_cast<uint16_t*>(ws), n8, n8};
     ws += align256(size_t(M) * n8 * 2);
   }
-  if (db || (make && (dx || dw))) {
+  const Rows rw = dx ? rows_of(w, ldw, K) : Rows();
+  const Epi to_dx = dx ? plain_epi(dx, dx_dtype == GD_F32, lddx) : Epi();
+  const bool together = dx && act != kNone && dy_dtype != GD_F32 && aligned(dy, 16) && lddy % 8 == 0 && aligned(z, 16) &&
+                        ldz % 8 == 0 && N % kR == 0 && K % 8 == 0 && dz_dx_fits(M, K, N) && !to_dx.y_f32 && to_dx.y_vec;
+  if (together) {
+    DzDx a = {};
+    a.dy = static_cast<const uint16_t*>(dy);
+    a.lddy = lddy;
+    a.z = static_cast<const uint16_t*>(z);
+    a.ldz = ldz;
+    a.w = rw.p;
+    a.ldw = rw.ld;
+    a.w_cols = rw.cols;
+    a.dz = dw ? const_cast<uint16_t*>(rz.p) : nullptr;
+    a.lddz = n8;
+    a.dx = static_cast<uint16_t*>(dx);
+    a.lddx = lddx;
+    a.M = M;
+    a.K = K;
+    a.N = N;
+    a.act = act;
+    const int blocks = int(div_up(M, kTogetherRows));
+    if (db) {
+      a.sums = reinterpret_cast<float*>(ws);
+      ws += align256(size_t(blocks) * N * sizeof(float));
+    }
+    if (K <= 128)
+      hipLaunchKernelGGL((linear_dz_dx<E, 2>), dim3(blocks), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((linear_dz_dx<E, 4>), dim3(blocks), dim3(256), 0, s, a);
+    GD_LAUNCH_CHECK("linear_dz_dx");
+    if (db) {
+      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(kSumThreads), 0, s, a.sums, blocks, N, db,
+                         int(param_dtype == GD_F32));
+      GD_LAUNCH_CHECK("linear_colsum");
+    }
+  } else if (db || (make && (dx || dw))) {
     const DactPlan d = dact_plan(M, N);
     Dact a = {};
     a.dy = dy;
@@ -1211,13 +1411,12 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     hipLaunchKernelGGL(linear_dact<E>, dim3(d.blocks, d.slabs), dim3(256), 0, s, a);
     GD_LAUNCH_CHECK("linear_dact");
     if (db) {
-      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(256), 0, s, a.sums, d.blocks, N,
+      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(kSumThreads), 0, s, a.sums, d.blocks, N,
                          db, int(param_dtype == GD_F32));
       GD_LAUNCH_CHECK("linear_colsum");
     }
   }
-  if (dx) {
-    const Rows rw = rows_of(w, ldw, K);
+  if (dx && !together) {
     Gemm g = {};
     g.a = rz.p;
     g.lda = rz.ld;
@@ -1228,7 +1427,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     g.cb = rw.cols;
     g.M = M;
     g.N = K;
-    g.epi = plain_epi(dx, dx_dtype == GD_F32, lddx);
+    g.epi = to_dx;
     const Plan p = plan_of(M, K, n8);
     GD_TRY((product<E, false, true>(p, g, ws, s)));
     ws += p.bytes;
@@ -1254,7 +1453,10 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
 size_t backward_bytes(int M, int K, int N, bool dx, bool dw, bool db) {
   const int n8 = pad8(N);
   size_t b = dx || dw ? align256(size_t(M) * n8 * 2) : 0;
-  if (db) b += align256(size_t(dact_plan(M, N).blocks) * N * sizeof(float));
+  if (db) {
+    const int64_t alone = dact_plan(M, N).blocks, together = dx && dz_dx_fits(M, K, N) ? div_up(M, kTogetherRows) : 0;
+    b += align256(size_t(alone > together ? alone : together) * N * sizeof(float));
+  }
   if (dx) b += plan_of(M, K, n8).bytes;
   if (dw) b += plan_of(N, K, M).bytes;
   return b;

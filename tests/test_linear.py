@@ -54,6 +54,22 @@ def test_workgroups_over_many_tiles(emulated, monkeypatch, groups, m, k, n, act,
     lc.check(x, w, b, act, r, y, dy, grads)
 
 
+@pytest.mark.parametrize("m,k,n,act,dtype", [(200, 256, 128, "relu", BF), (129, 96, 192, "gelu", HF), (64, 8, 64, "silu", BF),
+                                             (300, 136, 64, "gelu_tanh", BF)])
+def test_slope_and_product_together(emulated, monkeypatch, m, k, n, act, dtype):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", "1")
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, k != 8, None, seed=6)
+    y, grads = lc.run(x, w, b, act, r, dy)
+    lc.check(x, w, b, act, r, y, dy, grads)
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, True, None, seed=7)
+    w.requires_grad_(False)  # (dz itself is not kept)
+    b.requires_grad_(False)
+    from gdino_amd.linear import linear_act
+    y = linear_act(x, w, b, act)
+    dx, = torch.autograd.grad(y, [x], dy)
+    lc.check(x, w, b, act, None, y, dy, (dx, None, None, None))
+
+
 def test_strides_and_shapes(emulated):
     """Leading dimensions, transposed and sliced inputs, an expanded residual and gradient, a misaligned view."""
     from gdino_amd.linear import linear_act

@@ -50,6 +50,15 @@ def test_workgroups_over_many_tiles(monkeypatch, groups, m, k, n):
         lc.check(x, w, b, act, r, y, dy, grads)
 
 
+@pytest.mark.parametrize("m,k,n", [(200, 256, 128), (1000, 96, 384), (2051, 192, 768), (130, 8, 2048), (9001, 256, 2048)])
+def test_slope_and_product_together(monkeypatch, m, k, n):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", "1")
+    for dtype, act in ((BF, "relu"), (HF, "gelu_tanh"), (BF, "silu"), (HF, "gelu")):
+        x, w, b, r, dy = lc.inputs(m, k, n, dtype, act != "silu", None, seed=k, device="cuda")
+        y, grads = lc.run(x, w, b, act, r, dy)
+        lc.check(x, w, b, act, r, y, dy, grads)
+
+
 def test_large_values():
     """Activations far from zero: nothing overflows on the way to a finite result."""
     from gdino_amd.linear import linear_act
