@@ -189,9 +189,9 @@ __device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool ve
 
 // 16 bytes of an output, which nothing reads soon: past the caches' ways of lines that are kept
 // (16384 x 512 -> 4096: 112 us with plain stores, 102 with these; 44446 x 256 -> 2048: 108 and 98)
-__device__ __forceinline__ void st_out(uint16_t* p, uint4 u) {
+__device__ __forceinline__ void st_out(void* p, uint4 u) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-  GD_STORE_NT((u32x4{u.x, u.y, u.z, u.w}), reinterpret_cast<u32x4*>(p));
+  GD_STORE_NT((u32x4{u.x, u.y, u.z, u.w}), static_cast<u32x4*>(p));
 }
 
 template <typename E>
@@ -729,11 +729,12 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
                                      n0 + 16 * wn * T, split, lane);
 }
 
-// 16 rows of 64 columns from m, n on: lane (c, g) has the pieces of row c, columns 8 g and 32 + 8 g.  Lanes c and c ^ 1 trade
-// one, so that an instruction writes whole rows of 128 bytes (64 bytes of twice the rows take twice the time:
-// 199 us against 82 for 44446 x 256 -> 2048).
-__device__ __forceinline__ void write_rows(uint16_t* to, int64_t ld, int m, int n, int M, int N, int lane, uint4 first,
-                                           uint4 second) {
+// 16 rows from m on: lane (c, g) has two 16-byte pieces of row c, at bytes 16 g and 64 + 16 g of 128 (16-bit output, 64
+// columns; pitch `apart` 64) or at 32 g and 32 g + 16 (fp32 output, 32 columns; 16).  Lanes c and c ^ 1 trade one, so that
+// an instruction writes whole rows of 128 bytes (64 bytes of twice the rows take twice the time: 199 us against 82
+// for 44446 x 256 -> 2048).
+__device__ __forceinline__ void write_rows(char* row0, int64_t pitch, int at, int apart, int m, int M, int bytes, int lane,
+                                           uint4 first, uint4 second) {
   const bool odd = (lane & 1) != 0;
   const uint4 give = odd ? first : second;
   uint4 take;
@@ -742,10 +743,21 @@ __device__ __forceinline__ void write_rows(uint16_t* to, int64_t ld, int m, int 
   take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
   take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
   m += lane & 14;
-  n += 8 * (lane >> 4) + (odd ? 32 : 0);
-  uint16_t* const at = to + m * ld + n;
-  if (m < M && n < N) st_out(at, odd ? take : first);
-  if (m + 1 < M && n < N) st_out(at + ld, odd ? second : take);
+  at += odd ? apart : 0;
+  char* const to = row0 + m * pitch + at;
+  if (m < M && at < bytes) st_out(to, odd ? take : first);
+  if (m + 1 < M && at < bytes) st_out(to + pitch, odd ? second : take);
+}
+// 64 columns from n on, of 16 bits: the pieces of columns 8 g and 32 + 8 g
+__device__ __forceinline__ void write16(uint16_t* to, int64_t ld, int m, int n, int M, int N, int lane, uint4 first,
+                                        uint4 second) {
+  write_rows(reinterpret_cast<char*>(to), 2 * ld, 2 * n + 16 * (lane >> 4), 64, m, M, 2 * N, lane, first, second);
+}
+// 32 columns from n on, fp32: the pieces of columns 8 g and 8 g + 4
+__device__ __forceinline__ void write32(float* to, int64_t ld, int m, int n, int M, int N, int lane, const float v[8]) {
+  const uint4 first = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  const uint4 second = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+  write_rows(reinterpret_cast<char*>(to), 4 * ld, 4 * n + 32 * (lane >> 4), 16, m, M, 4 * N, lane, first, second);
 }
 
 // 128 x 128 tiles of a layer with few features in, by workgroups that go from tile to tile: the next tile's first two
@@ -875,10 +887,13 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] += p.epi.res_f32 ? raw.f[j] : E::up(raw.h16[j]);
           }
-          y[h] = pack8<E>(x);
+          if (p.epi.y_f32)
+            write32(static_cast<float*>(p.epi.y), p.epi.ldy, m0 + 16 * i, n0 + 32 * h, p.M, p.N, lane, x);
+          else
+            y[h] = pack8<E>(x);
         }
-        if (p.epi.z) write_rows(p.epi.z, p.epi.ldz, m0 + 16 * i, n0, p.M, p.N, lane, z[0], z[1]);
-        write_rows(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, m0 + 16 * i, n0, p.M, p.N, lane, y[0], y[1]);
+        if (p.epi.z) write16(p.epi.z, p.epi.ldz, m0 + 16 * i, n0, p.M, p.N, lane, z[0], z[1]);
+        if (!p.epi.y_f32) write16(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, m0 + 16 * i, n0, p.M, p.N, lane, y[0], y[1]);
       }
     };
     switch (p.epi.act) {
@@ -1116,7 +1131,7 @@ __global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
       for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * h + (j >> 2)][j & 3];
       x[h] = pack8<E>(v);
     }
-    write_rows(p.dx, p.lddx, m0 + 16 * (wm * TM + i), 64 * wn, p.M, p.K, lane, x[0], x[1]);
+    write16(p.dx, p.lddx, m0 + 16 * (wm * TM + i), 64 * wn, p.M, p.K, lane, x[0], x[1]);
   }
 }
 
@@ -1221,7 +1236,7 @@ Plan plan_of(int M, int N, int r) {
 
 // whether linear_stream takes a layer: whole chunks, at least two, and whole aligned pieces in every row
 bool streams(const Gemm& g) {
-  return g.ra == g.rb && g.ra % kR == 0 && g.ra >= 2 * kR && g.N % 8 == 0 && !g.epi.y_f32 && g.epi.y_vec &&
+  return g.ra == g.rb && g.ra % kR == 0 && g.ra >= 2 * kR && g.N % 8 == 0 && g.epi.y_vec &&
          (!g.epi.bias || g.epi.bias_vec) && (!g.epi.res || g.epi.res_vec);
 }
 
