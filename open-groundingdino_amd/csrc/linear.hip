@@ -1196,11 +1196,12 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Tile and parts of one product: the cheapest by a model of what was measured (us, 16-bit, 64 values of r at a time).
 // A round is as many tiles as run at once (1, 2 or 3 workgroups per CU, by their LDS); it costs `base` (the first loads
 // and the output) and `chunk` per 64 values of r, `alone` where a CU has one workgroup only:
-//   256 x 256  16384 x 4096 x 4096 in 4 rounds of 64 chunks: 425 us.  Only where 8 tiles or more share each operand's
-//              chunk: it waits for one chunk at a time, which has to come from L2 (44446 x 2048 x 256: 100 us, by 128s 59)
-//   128 x 128  the same 490 us in 8 rounds; 8400 x 1536 x 384 in one, 198 workgroups: 22 us
-//   64 x 64    900 x 256 x 2048 in one round of 480: 6.1 us (by 128s 8.7)
-// Parts of a split sum are written and read once more, in fp32 at about 4 TB/s, by a further launch.
+//   256 x 256  16384 x 4096 x 4096 in 4 rounds of 64 chunks: 425 us.  Only where 4 tiles or more share each operand's
+//              chunk: it waits for one chunk at a time, which has to come from L2 (44446 x 2048 x 256: 100 us, by 128s 56)
+//   128 x 128  the same 485 us in 8 rounds; 8400 x 1536 x 384 in one, 198 workgroups: 20 us
+//   64 x 64    900 x 256 x 256 in one round of 60: 4.6 us (by 128s 7.1)
+// Parts of a split sum are written and read once more, in fp32 at about 6 TB/s (they stay near), by a further launch.
+// Over 72 products of this detector's sizes the choice is 0.6 % off the best of the three on average, 10 % at most.
 struct Plan {
   int tile, splits, r_per_split;
   size_t bytes;
@@ -1210,18 +1211,18 @@ Plan plan_of(int M, int N, int r) {
     int tile, slots;
     double chunk, alone, base;
   };
-  constexpr Kind kinds[] = {{256, 256, 1.5, 1.5, 12.0}, {128, 512, 0.86, 0.65, 6.0}, {64, 768, 0.47, 0.35, 3.6}};
+  constexpr Kind kinds[] = {{256, 256, 1.5, 1.5, 11.5}, {128, 512, 0.80, 0.67, 5.0}, {64, 768, 0.55, 0.40, 2.9}};
   const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256)
   const int64_t chunks = div_up(r, kR);
   Plan p = {};
   double best = 1e30;
   for (const Kind& k : kinds) {
     const int64_t tm = div_up(M, k.tile), tn = div_up(N, k.tile);
-    if (forced ? forced != k.tile : (k.tile == 256 && (tm < 8 || tn < 8))) continue;
+    if (forced ? forced != k.tile : (k.tile == 256 && (tm < 4 || tn < 4))) continue;
     for (int64_t s = 1; s == 1 || (s <= 64 && chunks / s >= 4); s *= 2) {
       const int64_t part = div_up(chunks, s), parts = div_up(chunks, part), blocks = tm * tn * parts;
       double cost = double(div_up(blocks, k.slots)) * (double(part) * (blocks <= 256 ? k.alone : k.chunk) + k.base);
-      if (parts > 1) cost += 5.0 + double(parts) * M * N * 8.0 / 4e6;
+      if (parts > 1) cost += 3.4 + double(parts) * M * N * 8.0 / 6e6;
       if (cost < best) {
         best = cost;
         p.tile = k.tile;
