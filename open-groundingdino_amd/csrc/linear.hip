@@ -28,6 +28,7 @@ enum Act : int { kNone = 0, kRelu = 1, kGelu = 2, kGeluTanh = 3, kSilu = 4 };
 
 typedef short gd_i16x8 __attribute__((ext_vector_type(8)));
 typedef short gd_i16x4 __attribute__((ext_vector_type(4)));
+typedef float gd_f32x2 __attribute__((ext_vector_type(2)));
 typedef float gd_f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 gd_bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
@@ -50,6 +51,10 @@ typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
 struct Bf16 {
   static __device__ __forceinline__ float up(uint16_t h) { return bf16_to_f32(h); }
   static __device__ __forceinline__ uint16_t down(float f) { return f32_to_bf16(f); }
+  static __device__ __forceinline__ uint32_t down2(float a, float b) {  // (one instruction)
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(gd_f32x2{a, b}, bf16x2));
+  }
   static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf16x8, a), __builtin_bit_cast(gd_bf16x8, b),
                                                    c, 0, 0, 0);
@@ -64,6 +69,7 @@ struct Fp16 {
     const _Float16 h = (_Float16)f;
     return __builtin_bit_cast(uint16_t, h);
   }
+  static __device__ __forceinline__ uint32_t down2(float a, float b) { return down(a) | uint32_t(down(b)) << 16; }
   static __device__ __forceinline__ gd_f32x4 mma(gd_i16x8 a, gd_i16x8 b, gd_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gd_f16x8, a), __builtin_bit_cast(gd_f16x8, b), c,
                                                   0, 0, 0);
@@ -196,13 +202,7 @@ __device__ __forceinline__ void st_out(void* p, uint4 u) {
 
 template <typename E>
 __device__ __forceinline__ uint4 pack8(const float v[8]) {
-  union {
-    uint4 u;
-    uint16_t h[8];
-  } w;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
-  return w.u;
+  return make_uint4(E::down2(v[0], v[1]), E::down2(v[2], v[3]), E::down2(v[4], v[5]), E::down2(v[6], v[7]));
 }
 
 template <typename E, bool NT = true>
@@ -220,21 +220,15 @@ __device__ __forceinline__ void st8(void* p, int64_t at, bool f32, bool vec, int
     return;
   }
   uint16_t* q = static_cast<uint16_t*>(p) + at;
-  union {
-    uint4 u;
-    uint16_t h[8];
-  } w;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w.h[j] = E::down(v[j]);
   if (vec && left >= 8) {
     if (NT)
-      st_out(q, w.u);
+      st_out(q, pack8<E>(v));
     else
-      *reinterpret_cast<uint4*>(q) = w.u;
+      *reinterpret_cast<uint4*>(q) = pack8<E>(v);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) q[j] = w.h[j];
+      if (j < left) q[j] = E::down(v[j]);
   }
 }
 
