@@ -610,6 +610,112 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
                                        n0 + 16 * wn * TN, split, lane);
 }
 
+// 16 rows from m on: lane (c, g) has two 16-byte pieces of row c, at bytes 16 g and 64 + 16 g of 128 (16-bit output, 64
+// columns; pitch `apart` 64) or at 32 g and 32 g + 16 (fp32 output, 32 columns; 16).  Lanes c and c ^ 1 trade one, so that
+// an instruction writes whole rows of 128 bytes (64 bytes of twice the rows take twice the time: 199 us against 82
+// for 44446 x 256 -> 2048).
+__device__ __forceinline__ void write_rows(char* row0, int64_t pitch, int at, int apart, int m, int M, int bytes, int lane,
+                                           uint4 first, uint4 second) {
+  const bool odd = (lane & 1) != 0;
+  const uint4 give = odd ? first : second;
+  uint4 take;
+  take.x = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.x)));
+  take.y = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.y)));
+  take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
+  take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
+  m += lane & 14;
+  at += odd ? apart : 0;
+  char* const to = row0 + m * pitch + at;
+  if (m < M && at < bytes) st_out(to, odd ? take : first);
+  if (m + 1 < M && at < bytes) st_out(to + pitch, odd ? second : take);
+}
+// 64 columns from n on, of 16 bits: the pieces of columns 8 g and 32 + 8 g
+__device__ __forceinline__ void write16(uint16_t* to, int64_t ld, int m, int n, int M, int N, int lane, uint4 first,
+                                        uint4 second) {
+  write_rows(reinterpret_cast<char*>(to), 2 * ld, 2 * n + 16 * (lane >> 4), 64, m, M, 2 * N, lane, first, second);
+}
+// 32 columns from n on, fp32: the pieces of columns 8 g and 8 g + 4
+__device__ __forceinline__ void write32(float* to, int64_t ld, int m, int n, int M, int N, int lane, const float v[8]) {
+  const uint4 first = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  const uint4 second = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+  write_rows(reinterpret_cast<char*>(to), 4 * ld, 4 * n + 32 * (lane >> 4), 16, m, M, 4 * N, lane, first, second);
+}
+
+// A wave's T x 8 blocks (of operands read as PAIRS) with their epilogue, straight from the registers, one row of blocks after
+// the other (the accumulators are picked by comparison); the residual is asked for a row of blocks ahead.
+template <typename E, int T>
+__device__ __forceinline__ void store_direct(const Gemm& p, const gd_f32x4 (&acc)[T][8], int m0, int n0, int lane) {
+  const int c = lane & 15, g = lane >> 4;
+  uint4 bias[4], res[4][2];
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    const int n = n0 + 32 * h + 8 * g;
+    bias[h] = p.epi.bias ? *reinterpret_cast<const uint4*>(p.epi.bias + (n < p.N ? n : p.N - 8)) : make_uint4(0, 0, 0, 0);
+  }
+  const char* const from = static_cast<const char*>(p.epi.res);
+  const int64_t size = p.epi.res_f32 ? 4 : 2;
+  auto ask = [&](int i) {
+    const int m = m0 + 16 * i + c;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const int n = n0 + 32 * h + 8 * g;
+      const uint4* const r =
+          reinterpret_cast<const uint4*>(from + ((m < p.M ? m : p.M - 1) * p.epi.ldr + (n < p.N ? n : p.N - 8)) * size);
+      res[h][0] = r[0];
+      res[h][1] = r[p.epi.res_f32 ? 1 : 0];
+    }
+  };
+  if (from) ask(0);
+#pragma unroll 1
+  for (int i = 0; i < T; ++i) {
+    float x[4][8];
+#pragma unroll
+    for (int q = 0; q < T; ++q)
+      if (q == i) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[h][j] = acc[q][2 * h + (j >> 2)][j & 3];
+      }
+    uint4 z[4], y[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      union {
+        uint4 u[2];
+        uint16_t h16[16];
+        float f[8];
+      } b, r;
+      b.u[0] = bias[h];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[h][j] += E::up(b.h16[j]);
+      if (p.epi.z) z[h] = pack8<E>(x[h]);
+      activate8(x[h], p.epi.act);
+      if (from) {
+        r.u[0] = res[h][0];
+        r.u[1] = res[h][1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[h][j] += p.epi.res_f32 ? r.f[j] : E::up(r.h16[j]);
+      }
+    }
+    if (from) ask(i + 1 < T ? i + 1 : i);
+    const int m = m0 + 16 * i;
+    if (p.epi.z) {
+      write16(p.epi.z, p.epi.ldz, m, n0, p.M, p.N, lane, z[0], z[1]);
+      write16(p.epi.z, p.epi.ldz, m, n0 + 64, p.M, p.N, lane, z[2], z[3]);
+    }
+    if (p.epi.y_f32) {
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+        write32(static_cast<float*>(p.epi.y), p.epi.ldy, m, n0 + 32 * h, p.M, p.N, lane, x[h]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 4; ++h) y[h] = pack8<E>(x[h]);
+      write16(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, m, n0, p.M, p.N, lane, y[0], y[1]);
+      write16(static_cast<uint16_t*>(p.epi.y), p.epi.ldy, m, n0 + 64, p.M, p.N, lane, y[2], y[3]);
+    }
+  }
+}
+
 // 256 x 256 tiles of 4 waves, 128 x 128 each, one per SIMD: the largest wave tile its 512 registers allow, since LDS is
 // what the matrix cores compete for (128 KB are read and 64 KB written per chunk of 64 values of r; 8 waves of 128 x
 // 64 read 192 KB and wait for each other: 444 us at 16384 x 4096 x 4096, the products and reads alone 286, the
@@ -618,7 +724,10 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
 // LDS holds a ring of 5 images of one operand each, in the order A0 B0 A1 B1 A2 ...: A of chunk k + 2 is loaded in the
 // first phase of chunk k, to the image that B of chunk k - 1 left, B of chunk k + 2 in the second, to that of A of
 // chunk k: one load per 8 products, all the time.
-template <typename E, bool AC, bool BC>
+// DIRECT, a layer with whole pieces (`streams`): the output leaves straight from the registers (16384 x 4096 x 4096 with
+// tanh-GELU and residual: 449 us, through LDS 476; a gradient, without an epilogue, is as fast through LDS, and going on
+// to a next tile whose chunks are asked for before the output brought nothing, 450).
+template <typename E, bool AC, bool BC, bool DIRECT>
 __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   constexpr int T = 8, kWaves = 4, BX = 256, kImg = BX * kR, kRing = 5;
   constexpr int kOwn = store_floats<T>(4);
@@ -636,7 +745,8 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
 
   using Load = Loader<BX, AC, kWaves>;  // 8 instructions a wave and image
   Load la(p.a, p.lda, m0, p.M, p.ca, rb0, wave, lane);
-  Loader<BX, BC, kWaves> lb(p.b, p.ldb, n0, p.N, p.cb, rb0, wave, lane);
+  Loader<BX, BC, kWaves, DIRECT> lb(p.b, p.ldb, n0, p.N, p.cb, rb0, wave, lane);
+  static_assert(!DIRECT || (!AC && !BC), "a layer");
   static_assert(Load::kInstr == T, "one instruction per row of blocks");
 
   gd_f32x4 acc[T][T];
@@ -719,39 +829,11 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
   GD_MMA_WAIT8("s_nop 15\n\ts_nop 7", acc[0]);
 #pragma unroll
   for (int i = 1; i < T; ++i) GD_MMA_WAIT8("", acc[i]);
-  store_tile<E, T, T, 4, !AC && !BC>(p, acc, reinterpret_cast<float*>(lds) + wave * kOwn, m0 + 16 * wm * T,
-                                     n0 + 16 * wn * T, split, lane);
-}
-
-// 16 rows from m on: lane (c, g) has two 16-byte pieces of row c, at bytes 16 g and 64 + 16 g of 128 (16-bit output, 64
-// columns; pitch `apart` 64) or at 32 g and 32 g + 16 (fp32 output, 32 columns; 16).  Lanes c and c ^ 1 trade one, so that
-// an instruction writes whole rows of 128 bytes (64 bytes of twice the rows take twice the time: 199 us against 82
-// for 44446 x 256 -> 2048).
-__device__ __forceinline__ void write_rows(char* row0, int64_t pitch, int at, int apart, int m, int M, int bytes, int lane,
-                                           uint4 first, uint4 second) {
-  const bool odd = (lane & 1) != 0;
-  const uint4 give = odd ? first : second;
-  uint4 take;
-  take.x = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.x)));
-  take.y = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.y)));
-  take.z = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.z)));
-  take.w = __float_as_uint(dpp<DPP_XOR1>(__uint_as_float(give.w)));
-  m += lane & 14;
-  at += odd ? apart : 0;
-  char* const to = row0 + m * pitch + at;
-  if (m < M && at < bytes) st_out(to, odd ? take : first);
-  if (m + 1 < M && at < bytes) st_out(to + pitch, odd ? second : take);
-}
-// 64 columns from n on, of 16 bits: the pieces of columns 8 g and 32 + 8 g
-__device__ __forceinline__ void write16(uint16_t* to, int64_t ld, int m, int n, int M, int N, int lane, uint4 first,
-                                        uint4 second) {
-  write_rows(reinterpret_cast<char*>(to), 2 * ld, 2 * n + 16 * (lane >> 4), 64, m, M, 2 * N, lane, first, second);
-}
-// 32 columns from n on, fp32: the pieces of columns 8 g and 8 g + 4
-__device__ __forceinline__ void write32(float* to, int64_t ld, int m, int n, int M, int N, int lane, const float v[8]) {
-  const uint4 first = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-  const uint4 second = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
-  write_rows(reinterpret_cast<char*>(to), 4 * ld, 4 * n + 32 * (lane >> 4), 16, m, M, 4 * N, lane, first, second);
+  if constexpr (DIRECT)
+    store_direct<E, T>(p, acc, m0 + 16 * wm * T, n0 + 16 * wn * T, lane);
+  else
+    store_tile<E, T, T, 4, !AC && !BC>(p, acc, reinterpret_cast<float*>(lds) + wave * kOwn, m0 + 16 * wm * T,
+                                       n0 + 16 * wn * T, split, lane);
 }
 
 // 128 x 128 tiles of a layer with few features in, by workgroups that go from tile to tile: the next tile's first two
@@ -1248,9 +1330,12 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   if (!AC && plan.tile == 128 && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g)) {
     const int64_t at_once = env_int("GD_LINEAR_GROUPS", 512);
     hipLaunchKernelGGL((linear_stream<E, BC>), dim3(unsigned(grid < at_once ? grid : at_once)), dim3(256), 0, s, g);
-  } else if (plan.tile == 256)
-    hipLaunchKernelGGL((linear_gemm256<E, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
-  else if (plan.tile == 128)
+  } else if (plan.tile == 256) {
+    if (!AC && !BC && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g))
+      hipLaunchKernelGGL((linear_gemm256<E, false, false, true>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+    else
+      hipLaunchKernelGGL((linear_gemm256<E, AC, BC, false>), dim3(unsigned(grid)), dim3(256), 0, s, g);
+  } else if (plan.tile == 128)
     hipLaunchKernelGGL((linear_gemm<E, 2, 2, 4, 4, 2, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);
   else
     hipLaunchKernelGGL((linear_gemm<E, 2, 2, 2, 2, 3, AC, BC>), dim3(unsigned(grid)), dim3(256), 0, s, g);

@@ -54,6 +54,15 @@ def test_workgroups_over_many_tiles(emulated, monkeypatch, groups, m, k, n, act,
     lc.check(x, w, b, act, r, y, dy, grads)
 
 
+@pytest.mark.parametrize("m,k,n,act,dtype,residual", [(270, 128, 320, "gelu_tanh", BF, BF), (200, 64, 192, "silu", HF, F32),
+                                                      (257, 136, 64, "relu", BF, None)])
+def test_large_tiles_straight_from_registers(emulated, monkeypatch, m, k, n, act, dtype, residual):
+    monkeypatch.setenv("GD_LINEAR_TILE", "256")
+    x, w, b, r, dy = lc.inputs(m, k, n, dtype, act != "silu", residual, seed=8)
+    y, grads = lc.run(x, w, b, act, r, dy)
+    lc.check(x, w, b, act, r, y, dy, grads)
+
+
 @pytest.mark.parametrize("m,k,n,act,dtype", [(200, 256, 128, "relu", BF), (129, 96, 192, "gelu", HF), (64, 8, 64, "silu", BF),
                                              (300, 136, 64, "gelu_tanh", BF)])
 def test_slope_and_product_together(emulated, monkeypatch, m, k, n, act, dtype):

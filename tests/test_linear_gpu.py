@@ -50,6 +50,15 @@ def test_workgroups_over_many_tiles(monkeypatch, groups, m, k, n):
         lc.check(x, w, b, act, r, y, dy, grads)
 
 
+@pytest.mark.parametrize("m,k,n", [(1100, 192, 1280), (513, 1024, 192), (256, 64, 264)])
+def test_large_tiles_straight_from_registers(monkeypatch, m, k, n):
+    monkeypatch.setenv("GD_LINEAR_TILE", "256")
+    for dtype, act, residual in ((BF, "relu", None), (HF, "gelu_tanh", HF), (BF, "silu", F32), (BF, "none", BF)):
+        x, w, b, r, dy = lc.inputs(m, k, n, dtype, act != "silu", residual, seed=k, device="cuda")
+        y, grads = lc.run(x, w, b, act, r, dy)
+        lc.check(x, w, b, act, r, y, dy, grads)
+
+
 @pytest.mark.parametrize("m,k,n", [(200, 256, 128), (1000, 96, 384), (2051, 192, 768), (130, 8, 2048), (9001, 256, 2048)])
 def test_slope_and_product_together(monkeypatch, m, k, n):
     monkeypatch.setenv("GD_LINEAR_TOGETHER", "1")
