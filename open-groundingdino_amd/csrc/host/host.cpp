@@ -392,6 +392,15 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
       ls = list_of(what, "steps", steps, {at::kFloat}, &device, false, &ones);
     }
     if (lp.held.empty()) Py_RETURN_NONE;
+    // (a list given twice; within a list any overlap is found above)
+    for (size_t i = 0; i < size->size(); ++i) {
+      if ((*size)[i] == 0) continue;
+      const uint64_t of[] = {lp.at[i], lg.at[i], lm.at[i], lv.at[i], eight ? lms.at[i] : 0, eight ? lvs.at[i] : 0,
+                             copies != Py_None ? lc.at[i] : 0};
+      for (int a = 0; a < 7; ++a)
+        for (int b = 0; b < a; ++b)
+          TORCH_CHECK_VALUE(of[a] == 0 || of[a] != of[b], what, ": two lists share tensor ", i);
+    }
     const Tensor lrt = tensor_of(lr_dev), nt = tensor_of(norm);
     const float* lrp = lrt.defined() ? scalar_of(what, "lr", lrt, *device) : nullptr;
     const float* np = nt.defined() ? scalar_of(what, "total_norm", nt, *device) : nullptr;
@@ -402,8 +411,9 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
                        eight ? lvs.at.data() : nullptr, copies != Py_None ? lc.at.data() : nullptr,
                        steps != Py_None ? ls.at.data() : nullptr, step, lr, lrp, b1, b2, eps, decay, np, max_norm, seed,
                        stream_of(lp.held[0])));
-    for (const Tensor& t : lp.held) t.unsafeGetTensorImpl()->bump_version();
-    for (const Tensor& t : lc.held) t.unsafeGetTensorImpl()->bump_version();
+    for (const List* list : std::initializer_list<const List*>{&lp, &lc})
+      for (const Tensor& t : list->held)
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();  // (inference tensors have none)
     Py_RETURN_NONE;
   });
 }

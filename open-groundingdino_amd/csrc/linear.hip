@@ -18,6 +18,7 @@
 // by bit.
 #include "gd_common.h"
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -1328,7 +1329,7 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   const int64_t grid = int64_t(g.tiles_m) * g.tiles_n * plan.splits;
   GD_REQUIRE(grid < (int64_t(1) << 31), "linear: grid too large");
   if (!AC && plan.tile == 128 && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g)) {
-    const int64_t at_once = env_int("GD_LINEAR_GROUPS", 512);
+    const int64_t at_once = std::max(1, env_int("GD_LINEAR_GROUPS", 512));  // (A/B) two of a CU
     hipLaunchKernelGGL((linear_stream<E, BC>), dim3(unsigned(grid < at_once ? grid : at_once)), dim3(256), 0, s, g);
   } else if (plan.tile == 256) {
     if (!AC && !BC && plan.splits == 1 && env_int("GD_LINEAR_STREAM", 1) && streams(g))
@@ -1449,7 +1450,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
   const Rows rw = dx ? rows_of(w, ldw, K) : Rows();
   const Epi to_dx = dx ? plain_epi(dx, dx_dtype == GD_F32, lddx) : Epi();
   const bool together = dx && act != kNone && dy_dtype != GD_F32 && aligned(dy, 16) && lddy % 8 == 0 && aligned(z, 16) &&
-                        ldz % 8 == 0 && N % kR == 0 && K % 8 == 0 && dz_dx_fits(M, K, N) && !to_dx.y_f32 && to_dx.y_vec;
+                        ldz % 8 == 0 && lddy <= kMaxPitch && ldz <= kMaxPitch && N % kR == 0 && K % 8 == 0 && dz_dx_fits(M, K, N) && !to_dx.y_f32 && to_dx.y_vec;
   if (together) {
     DzDx a = {};
     a.dy = static_cast<const uint16_t*>(dy);

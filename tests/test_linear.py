@@ -203,6 +203,30 @@ def test_refusals(emulated):
         _lib.call("gd_linear_forward", *split, None, 0, None)
 
 
+def test_rows_and_packing(emulated):
+    """What the products read as it is, the copies of the rest, and the refusal of a call without them."""
+    import ctypes
+    from gdino_amd import _lib
+    fn = _lib.lib().gd_linear_readable
+    fn.restype, fn.argtypes = ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int]
+    a = torch.randn(5, 24).to(BF)
+    at = a.data_ptr()
+    assert fn(at, 24, 24, 0) and fn(at, 24, 16, 0) and fn(at, 24, 17, 1)
+    assert not fn(at, 24, 17, 0) and not fn(at + 2, 24, 16, 0) and not fn(at, 23, 16, 0) and not fn(at, 16, 17, 1)
+    assert not fn(at, 1 << 23, 8, 0)
+    b = torch.randn(3, 20).to(BF)
+    out_a, out_b = torch.full((5, 16), 9.0).to(BF), torch.full((3, 16), 9.0).to(BF)
+    _lib.call("gd_linear_pack", at + 2, 24, 5, b.data_ptr(), 20, 3, 11, out_a.data_ptr(), out_b.data_ptr(), None)
+    for out, rows in ((out_a, a[:, 1:12]), (out_b, b[:, :11])):
+        assert torch.equal(out[:, :11], rows) and not out[:, 11:].any()
+    with pytest.raises(_lib.GdError, match="first matrix"):
+        _lib.call("gd_linear_pack", at, 8, 5, None, 0, 0, 11, out_a.data_ptr(), None, None)
+    y = torch.empty(5, 3).to(BF)
+    geo = (at + 2, 24, b.data_ptr(), 24, None, 0, None, 2, 0, 5, 16, 3)
+    with pytest.raises(_lib.GdError, match="16-byte pieces"):
+        _lib.call("gd_linear_forward", 2, *geo, y.data_ptr(), 2, 3, None, 0, 0, None, 0, None)
+
+
 def test_cpu_tensors_raise():
     from gdino_amd.linear import linear_act
     x, w, b, _, _ = lc.inputs(6, 24, 16, BF, grad=False)

@@ -187,3 +187,51 @@ def test_feed_forward_and_update_together():
         c.zero_grad()
         for p, q in zip(ours, theirs):  # an update moves a weight by about lr, whichever way a tiny gradient rounds
             assert float((p - q).detach().abs().max()) <= 2.5e-3 * (i + 1)
+
+
+def test_train_step_in_a_graph():
+    """Forward, gradients, their norm and the update as one captured graph, replayed beside the same steps run eagerly."""
+    from gdino_amd import optim
+    from gdino_amd.linear import mlp
+
+    def make():
+        torch.manual_seed(3)
+        layers = torch.nn.Linear(64, 256, dtype=BF).cuda(), torch.nn.Linear(256, 64, dtype=BF).cuda()
+        weights = [p for m in layers for p in m.parameters()]
+        return layers, weights, optim.AdamW(weights, lr=torch.tensor(1e-2, device="cuda"), state_bits=8, seed=5)
+
+    x = torch.zeros(300, 64, device="cuda", dtype=BF)
+    target = torch.randn(300, 64, device="cuda")
+
+    def step(layers, weights, opt):
+        grads = torch.autograd.grad((mlp(x, *layers).float() - target).square().mean(), weights)
+        for p, g in zip(weights, grads):
+            p.grad = g
+        opt.step(max_norm=0.5)
+        return opt.total_norm
+
+    inputs = [torch.randn(300, 64, device="cuda").to(BF) for _ in range(5)]
+    eager, want = make(), []
+    for t in inputs:
+        x.copy_(t)
+        norm = step(*eager)
+        want.append([norm.clone()] + [p.detach().clone() for p in eager[1]])
+    ours = make()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        x.copy_(inputs[0])
+        first = [step(*ours).clone()] + [p.detach().clone() for p in ours[1]]
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = step(*ours)
+    got = [first]
+    for t in inputs[1:]:
+        x.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        got.append([norm.clone()] + [p.detach().clone() for p in ours[1]])
+    for a, b in zip(got, want):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)

@@ -123,6 +123,9 @@ def test_refusals(emulated):
         step([p[0], p[0]], g, m, v)
     with pytest.raises(ValueError, match="overlap"):
         step(p, g, [m[0], m[0]], v)
+    for lists in ((p, g, m, m), (p, p, m, v), (p, g, p, v)):
+        with pytest.raises(ValueError, match="share tensor 0"):
+            step(*lists)
     with pytest.raises(ValueError, match="1 gradients for 2"):
         step(p, g[:1], m, v)
     with pytest.raises(ValueError, match="numbers of elements"):
@@ -165,6 +168,17 @@ def test_refusals(emulated):
         sizes = np.array([8], dtype=np.int64)
         addr = np.array([p[0].data_ptr()], dtype=np.uint64)
         _lib.call("gd_grad_norm", 1, sizes.tobytes(), 0, addr.tobytes(), None, 0, p[1].data_ptr(), None)
+
+
+def test_inference_tensors(emulated):
+    """Tensors without a version counter are updated like others."""
+    from gdino_amd import optim
+    want = oc.make([40])
+    with torch.inference_mode():
+        got = oc.make([40])
+        optim.adamw_step(*got, 1, **oc.HYPER)
+    optim.adamw_step(*want, 1, **oc.HYPER)
+    assert torch.equal(got[0][0], want[0][0]) and want[0][0]._version > 0
 
 
 def test_cpu_tensors_raise():
