@@ -208,9 +208,12 @@ def call(name: str, *args, flops: float | None = None, nbytes: float | None = No
     """Run entry point ``name``; raise GdError on a non-OK status.  ``flops``
     (MFMA entry points) and ``nbytes`` (HBM-bound ones), both algorithmic,
     feed CallTimer's TFLOP/s and GB/s."""
+    fn = getattr(lib(), name)
+    if getattr(fn, "argtypes", ()) is None:  # (ctypes would hand over 64-bit addresses as 32-bit integers)
+        raise GdError(f"{name}: no declared signature; import the module that registers it")
     timer = call_timer
     start = timer.begin() if timer is not None else None
-    status = getattr(lib(), name)(*args)
+    status = fn(*args)
     if status != GD_OK:
         msg = lib().gd_last_error().decode(errors="replace")
         raise GdError(f"{name}: status {status}: {msg}")

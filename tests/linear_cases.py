@@ -99,3 +99,39 @@ def run(x, w, b, act, r, dy):
     leaves = [t for t in (x, w, b, r) if t is not None]
     got = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, dy)))
     return y, tuple(None if t is None else got[id(t)] for t in (x, w, b, r))
+
+
+def check_around(device, m=333, k=136, n=192, pad=24):
+    """Outputs inside larger buffers: the columns beside them (y, dx with a pitch) and what follows stay as they were."""
+    import ctypes
+    import gdino_amd.linear  # noqa: F401  (declares the entry points)
+    from gdino_amd import _lib
+    x, w, b, _, dy = inputs(m, k, n, torch.bfloat16, seed=4, device=device, grad=False)
+    stream = _lib.stream_of(x) if device == "cuda" else None
+
+    def guarded(rows, cols, dtype=torch.bfloat16, beside=pad):
+        return torch.full((rows + 40, cols + beside), 7.0, dtype=dtype, device=device)
+
+    def inside(t, rows, cols):
+        got = t[:rows, :cols].clone()
+        t[:rows, :cols] = 7.0
+        assert (t == 7).all()
+        return got
+
+    fn = _lib.lib().gd_linear_backward_workspace_bytes
+    fn.restype, fn.argtypes = ctypes.c_size_t, [ctypes.c_int] * 6
+    for y_type, code in ((torch.bfloat16, 2), (torch.float32, 0)):
+        r = None if code else torch.zeros(m, n, device=device)
+        y, z = guarded(m, n, y_type), guarded(m, n, beside=0)
+        ws = torch.empty(1 << 22, dtype=torch.uint8, device=device)
+        _lib.call("gd_linear_forward", 2, x.data_ptr(), k, w.data_ptr(), k, b.data_ptr(), 2, _lib.ptr(r), code, n, m, k, n,
+                  y.data_ptr(), code, n + pad, z.data_ptr(), n, 0, ws.data_ptr(), ws.numel(), stream)
+        dx, dw, db = guarded(m, k), guarded(n, k, beside=0), guarded(1, n, beside=0)
+        nbytes = fn(m, k, n, 1, 1, 1)
+        ws = torch.full((nbytes + 4096,), 7, dtype=torch.uint8, device=device)
+        zs = inside(z, m, n)
+        _lib.call("gd_linear_backward", 2, 2, dy.data_ptr(), 2, n, zs.data_ptr(), n, x.data_ptr(), k, w.data_ptr(), k, m, k, n,
+                  dx.data_ptr(), 2, k + pad, dw.data_ptr(), db.data_ptr(), 2, 0, ws.data_ptr(), nbytes, stream)
+        assert (ws[nbytes:] == 7).all()
+        grads = inside(dx, m, k), inside(dw, n, k), inside(db, 1, n)[0], None
+        check(x, w, b, "gelu", r, inside(y, m, n), dy, grads)

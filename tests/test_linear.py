@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import emu_product
+import gdino_amd.linear  # noqa: F401  (declares the entry points that are called below)
 import linear_cases as lc
 
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -225,6 +226,20 @@ def test_rows_and_packing(emulated):
     geo = (at + 2, 24, b.data_ptr(), 24, None, 0, None, 2, 0, 5, 16, 3)
     with pytest.raises(_lib.GdError, match="16-byte pieces"):
         _lib.call("gd_linear_forward", 2, *geo, y.data_ptr(), 2, 3, None, 0, 0, None, 0, None)
+
+
+@pytest.mark.parametrize("tile,together", [("64", "1000000000"), ("128", "1"), ("256", "1000000000")])
+def test_nothing_around_the_outputs_is_written(emulated, monkeypatch, tile, together):
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_around("cpu")
+
+
+def test_undeclared_entry_points_are_refused(emulated):
+    """A call before its module declared the signature would cut the addresses to 32 bits."""
+    from gdino_amd import _lib
+    with pytest.raises(_lib.GdError, match="no declared signature"):
+        _lib.call("gd_linear_forward_workspace_bytes", 1, 1, 1)
 
 
 def test_cpu_tensors_raise():

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import linear_cases as lc
+import gdino_amd.linear  # noqa: F401  (declares the entry points that are called below)
 
 pytestmark = pytest.mark.gpu
 BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
@@ -152,6 +153,14 @@ def test_rows_behind_the_last_are_left():
               y.data_ptr(), 2, n, None, 0, 0, None, 0, _lib.stream_of(y))
     assert (y[m * n:] == 7).all()
     lc.check(x, w, b, "none", None, y[:m * n].view(m, n))
+
+
+@pytest.mark.parametrize("together", ["1", "1000000000"])
+@pytest.mark.parametrize("tile", ["64", "128", "256"])
+def test_nothing_around_the_outputs_is_written(monkeypatch, tile, together):
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_around("cuda")
 
 
 def test_feed_forward_and_update_together():
