@@ -36,6 +36,9 @@ constexpr int kOpVec = 4;                         // consecutive elements per la
 constexpr int kOpChunk = kOpThreads * kOpVec;
 constexpr uint32_t kOpPiece = 1u << 30;           // elements of one table entry at most
 constexpr uint32_t kOpAligned = 1u << 31;         // flag on an entry's count: vector accesses are aligned
+constexpr uint32_t kOpFirst = kOpPiece - 1;       // an entry's first workgroup; the bits above: its first element within
+                                                  // its tensor, a multiple of kOpPiece, modulo 2^32
+constexpr uint32_t kOpBlocks = 1u << 23;          // workgroups after which a launch is closed (its threads fit 32 bits)
 constexpr int kOpArgBytes = 3840;                 // the table's share of the 4 KB of kernel arguments
 
 // The table entry whose chunks hold workgroup b: `first` ascends from 0, so it is the number of entries
@@ -44,7 +47,7 @@ __device__ __forceinline__ int find_entry(const uint32_t* first, int n, uint32_t
   const int lane = threadIdx.x & 63;
   int at = -1;
   for (int i = 0; i < n; i += 64) {
-    const bool here = i + lane < n && first[i + lane] <= b;
+    const bool here = i + lane < n && (first[i + lane] & kOpFirst) <= b;
     at += __popcll(__ballot(here));
   }
   return at;
@@ -178,7 +181,7 @@ struct AdamConst {
 // E8: 8-bit moments, CP: a bf16 copy of the weights, ST: the step counts are on the device
 template <bool E8, bool CP, bool ST>
 struct AdamTable {
-  static constexpr int kEntry = 32 + (E8 ? 16 : 0) + (CP ? 8 : 0) + (ST ? 8 : 0) + (E8 ? 4 : 0) + 8;
+  static constexpr int kEntry = 32 + (E8 ? 16 : 0) + (CP ? 8 : 0) + (ST ? 8 : 0) + 8;
   static constexpr int kCap = kOpArgBytes / kEntry;
   float* p[kCap];
   const void* g[kCap];
@@ -188,14 +191,13 @@ struct AdamTable {
   uint8_t* vs[E8 ? kCap : 1];
   uint16_t* copy[CP ? kCap : 1];
   const float* step[ST ? kCap : 1];
-  uint32_t base[E8 ? kCap : 1];  // the entry's first element within its tensor
-  uint32_t n[kCap];              // elements | kOpAligned
-  uint32_t first[kCap];          // its first workgroup
+  uint32_t n[kCap];      // elements | kOpAligned
+  uint32_t first[kCap];  // see kOpFirst
   int entries;
 };
 
 // The hardware's root and reciprocal, an ulp each: exact ones are some 20 instructions per weight (8-bit moments:
-// 245 us -> 212 with one group of four per thread, detector).  The root takes denormal values for 0: scaled around it.
+// 245 us -> 212 for the detector).  The root takes denormal values for 0: scaled around it.
 __device__ __forceinline__ float op_sqrt(float x) {
   const bool tiny = x < 0x1p-96f;
   const float r = __builtin_amdgcn_sqrtf(tiny ? x * 0x1p96f : x);
@@ -242,7 +244,7 @@ __device__ __forceinline__ void adamw_four(const AdamTable<E8, CP, ST>& t, const
     uint32_t rm[4], rv[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t h = op_hash(t.base[e] + i + j, s.key);
+      const uint32_t h = op_hash((t.first[e] & ~kOpFirst) + i + j, s.key);
       rm[j] = h & 0xffffu;
       rv[j] = h >> 16;
       if (j >= k) m[j] = root[j] = 0.f;
@@ -268,7 +270,7 @@ adamw_kernel(const AdamTable<E8, CP, ST> t, const AdamConst c) {
   const int e = find_entry(t.first, t.entries, blockIdx.x);
   const bool vec = (t.n[e] & kOpAligned) != 0;
   const uint32_t n = t.n[e] & ~kOpAligned;
-  const uint32_t begin = (blockIdx.x - t.first[e]) * uint32_t(kOpChunk);
+  const uint32_t begin = (blockIdx.x - (t.first[e] & kOpFirst)) * uint32_t(kOpChunk);
 
   AdamStep s;
   float inv_bc1 = c.inv_bc1;
@@ -333,7 +335,6 @@ gd_status adamw_launch(int tensors, const AdamLists& l, const AdamConst& c, hipS
         t.v[e] = at<uint8_t>(l.v, i) + off;
         t.ms[e] = at<uint8_t>(l.ms, i) + off / 32;
         t.vs[e] = at<uint8_t>(l.vs, i) + off / 32;
-        t.base[e] = uint32_t(off);
         al = al && op_aligned(t.m[e], 4) && op_aligned(t.v[e], 4);
       } else {
         t.m[e] = at<float>(l.m, i) + off;
@@ -346,10 +347,9 @@ gd_status adamw_launch(int tensors, const AdamLists& l, const AdamConst& c, hipS
       }
       if constexpr (ST) t.step[e] = at<const float>(l.step, i);
       t.n[e] = n | (al ? kOpAligned : 0u);
-      t.first[e] = blocks;
+      t.first[e] = blocks | uint32_t(off);
       blocks += (n + kOpChunk - 1) / kOpChunk;
-      // a launch's grid stays far below 2^31 workgroups: 96 entries of 2^18 chunks
-      if (t.entries == AdamTable<E8, CP, ST>::kCap) {
+      if (t.entries == AdamTable<E8, CP, ST>::kCap || blocks >= kOpBlocks) {
         const gd_status st = flush();
         if (st != GD_OK) return st;
       }
