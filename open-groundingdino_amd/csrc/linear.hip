@@ -3,9 +3,13 @@
 //   z = x W^T + b     y = act(z) + r          x [M, K], W [N, K], bf16 / fp16
 //   dz = dy * act'(z)     dx = dz W     dW = dz^T x     db = sum_m dz     (dr = dy)
 //
-// All three products are one kernel, C[m][n] = sum_r A(m, r) B(n, r), whose
-// operands lie in memory either with r contiguous ("rows": x, W, dz in the
-// forward and dx) or with m / n contiguous ("columns": W in dx, dz and x in dW).
+// All three products are C[m][n] = sum_r A(m, r) B(n, r), whose operands lie in
+// memory either with r contiguous ("rows": x, W, dz in the forward and dx) or with
+// m / n contiguous ("columns": W in dx, dz and x in dW).  `plan_of` chooses the tile:
+//   linear_gemm      64 x 64 and 128 x 128, any layout and edge; dW, small and ragged layers
+//   linear_stream    128 x 128, workgroups that go from tile to tile; layers and dx of whole pieces
+//   linear_gemm256   256 x 256; large products, bound by the LDS that feeds the matrix cores
+//   linear_dz_dx     the activation's slope and dx in one, where memory is what costs
 // Products of 16-bit values are exact in fp32 and the accumulators are fp32
 // matrix-core registers; bias, activation and residual are applied to them in
 // fp32 and the result is rounded once.  The backward rounds dz to 16 bits, as the
@@ -535,7 +539,10 @@ __device__ __forceinline__ void store_tile(const Gemm& p, const gd_f32x4 (&acc)[
   }
 }
 
-// WM x WN waves, each of TM x TN blocks of 16 x 16; a ring of ST images, ST - 1 chunks of r in flight
+// WM x WN waves, each of TM x TN blocks of 16 x 16; a ring of ST images, ST - 1 chunks of r in flight.  64 x 64 tiles with 3
+// images (48 KB, three workgroups per CU): 900 x 256 x 256 4.6 us, latency; 128 x 128 with 2 (64 KB, two): dW of 44446 x
+// 256 x 2048 54 us (870 TFLOP/s), 16384 x 4096 x 4096 485 us (1.13 PFLOP/s), both by LDS, 96 KB in and out per chunk and
+// 512 products' worth of cycles.  Chunks of 32 values double the requests to L2 and were slower.
 template <typename E, int WM, int WN, int TM, int TN, int ST, bool AC, bool BC>
 __global__ void __launch_bounds__(64 * WM * WN) linear_gemm(const Gemm p) {
   constexpr int kWaves = WM * WN, BM = 16 * WM * TM, BN = 16 * WN * TN;
@@ -837,10 +844,11 @@ __global__ void __launch_bounds__(256, 1) linear_gemm256(const Gemm p) {
                                        n0 + 16 * wn * T, split, lane);
 }
 
-// 128 x 128 tiles of a layer with few features in, by workgroups that go from tile to tile: the next tile's first two
-// chunks are asked for before the output is stored, straight from the registers (a lane holds 8 consecutive
-// columns of a row), so loads, products and stores of the two workgroups of a CU run side by side.  For whole pieces
-// only (see `streams`).
+// 128 x 128 tiles by workgroups that go from tile to tile: the next tile's first two chunks are asked for before the output
+// is stored, straight from the registers (a lane holds 8 consecutive columns of a row), so loads, products and stores
+// of the two workgroups of a CU run side by side.  It matters for layers with few features in, whose tiles are short:
+// 44446 x 256 -> 2048 with ReLU 82 us (one tile per workgroup and outputs through LDS 98), 33400 x 192 -> 768 21 (30),
+// 16384 x 512 -> 4096 84 (99); with many features it is no slower.  For whole pieces only (see `streams`).
 template <typename E, bool BC>
 __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
   constexpr int T = 4, kWaves = 4, BX = 128, kStage = 2 * BX * kR;
@@ -1009,6 +1017,8 @@ __global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ p
 }
 
 // ---- dz = dy * act'(z), and parts of its column sums -------------------------------
+// A stream: 44446 x 2048 with ReLU, 546 MB, 108 us (5.1 TB/s).  dz is stored plainly: past the caches it costs the products
+// that read it next more than it saves here (the layer with its gradients 352 us instead of 342).
 struct Dact {
   const void* dy;
   const uint16_t* z;  // NULL: no activation
@@ -1064,14 +1074,12 @@ __global__ void __launch_bounds__(256) linear_dact(const Dact p) {
   }
 }
 
-// db[n] = sum of `parts` rows; 32 columns and 8 groups of rows per workgroup, the groups' sums added in order
 // dz = dy * act'(z) and dx = dz W together, for layers with up to 256 features in: a workgroup's tile of dx has all of
 // its columns, so dy and z are read once, and dz is not read back for dx (it is written where dW needs it).  A
 // chunk's dy and z are asked for a chunk ahead, into registers; their dz goes to LDS as the product's operand A, while
 // W's chunk comes by LDS-DMA.  64 rows by 64 WN columns: small, so that three workgroups of a CU wait for memory in turn
 // (128 rows need more registers than two workgroups of a CU have: 349 us against 125 for 44446 x 256 <- 2048, which
 // moves 570 MB; apart the two take 190, since dz's way out goes on while it is read back).
-constexpr int kSumThreads = 1024;
 struct DzDx {
   const uint16_t *dy, *z, *w;
   uint16_t *dz, *dx;  // dz: or NULL
@@ -1212,6 +1220,9 @@ __global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
   }
 }
 
+// db[n] = sum of `parts` rows; 32 columns and 32 groups of rows per workgroup, the groups' sums added in order (695 rows
+// of 2048: 6.6 us, all of it the loads' latency)
+constexpr int kSumThreads = 1024;
 template <typename E>
 __global__ void __launch_bounds__(kSumThreads) linear_colsum(const float* __restrict__ sums, int parts, int N,
                                                      void* __restrict__ db, int f32) {
