@@ -992,9 +992,47 @@ __global__ void __launch_bounds__(256, 2) linear_stream(const Gemm p) {
   }
 }
 
-// the parts added in order, then the epilogue; a thread per 8 columns
+// db[n] = sum of `parts` rows of column sums; 8 columns and 32 groups of rows per workgroup, the groups' sums added in order
+struct Join {
+  const float* sums;  // [parts][N]
+  void* db;
+  int parts, N, f32;
+  int first;          // the first workgroup that does this (of linear_finish)
+};
+constexpr int kJoinColumns = 8;
 template <typename E>
-__global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ part, int splits, int M, int N, Epi epi) {
+__device__ __forceinline__ void join_sums(const Join& j, int block) {
+  constexpr int kGroups = 256 / kJoinColumns;
+  __shared__ float lds[kGroups][kJoinColumns];
+  const int c = threadIdx.x % kJoinColumns, g = threadIdx.x / kJoinColumns;
+  const int n = block * kJoinColumns + c;
+  float s = 0.f;
+  if (n < j.N) {
+#pragma unroll 8
+    for (int k = g; k < j.parts; k += kGroups) s += j.sums[int64_t(k) * j.N + n];
+  }
+  lds[g][c] = s;
+  __syncthreads();
+  if (g == 0 && n < j.N) {
+    for (int k = 1; k < kGroups; ++k) s += lds[k][c];
+    if (j.f32)
+      static_cast<float*>(j.db)[n] = s;
+    else
+      static_cast<uint16_t*>(j.db)[n] = E::down(s);
+  }
+}
+template <typename E>
+__global__ void __launch_bounds__(256) linear_colsum(const Join j) {
+  join_sums<E>(j, int(blockIdx.x));
+}
+
+// the parts added in order, then the epilogue; a thread per 8 columns.  Further workgroups join column sums (a launch less)
+template <typename E>
+__global__ void __launch_bounds__(256) linear_finish(const float* __restrict__ part, int splits, int M, int N, Epi epi, Join join) {
+  if (int(blockIdx.x) >= join.first) {
+    join_sums<E>(join, int(blockIdx.x) - join.first);
+    return;
+  }
   const int per_row = (N + 7) / 8;
   const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
   if (i >= int64_t(M) * per_row) return;
@@ -1220,32 +1258,6 @@ __global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
   }
 }
 
-// db[n] = sum of `parts` rows; 32 columns and 32 groups of rows per workgroup, the groups' sums added in order (695 rows
-// of 2048: 6.6 us, all of it the loads' latency)
-constexpr int kSumThreads = 1024;
-template <typename E>
-__global__ void __launch_bounds__(kSumThreads) linear_colsum(const float* __restrict__ sums, int parts, int N,
-                                                     void* __restrict__ db, int f32) {
-  constexpr int kGroups = kSumThreads / 32;
-  __shared__ float lds[kGroups][32];
-  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int n = int(blockIdx.x) * 32 + c;
-  float s = 0.f;
-  if (n < N) {
-#pragma unroll 8
-    for (int k = g; k < parts; k += kGroups) s += sums[int64_t(k) * N + n];
-  }
-  lds[g][c] = s;
-  __syncthreads();
-  if (g == 0 && n < N) {
-    for (int k = 1; k < kGroups; ++k) s += lds[k][c];
-    if (f32)
-      static_cast<float*>(db)[n] = s;
-    else
-      static_cast<uint16_t*>(db)[n] = E::down(s);
-  }
-}
-
 // ---- rows that are not 16-byte aligned, copied with their ends filled with zeros; two matrices in one launch ------
 struct Pack {
   const uint16_t* src[2];
@@ -1330,7 +1342,7 @@ bool streams(const Gemm& g) {
 }
 
 template <typename E, bool AC, bool BC>
-gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
+gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s, Join join = Join()) {
   g.splits = plan.splits;
   g.r_per_split = plan.r_per_split;
   g.part = static_cast<float*>(part);
@@ -1354,8 +1366,11 @@ gd_status product(const Plan& plan, Gemm g, void* part, hipStream_t s) {
   GD_LAUNCH_CHECK("linear_gemm");
   if (plan.splits > 1) {
     const int64_t blocks = div_up(int64_t(g.M) * ((g.N + 7) / 8), 256);
-    GD_REQUIRE(blocks < (int64_t(1) << 31), "linear: grid too large");
-    hipLaunchKernelGGL(linear_finish<E>, dim3(unsigned(blocks)), dim3(256), 0, s, g.part, plan.splits, g.M, g.N, g.epi);
+    GD_REQUIRE(blocks < (int64_t(1) << 30), "linear: grid too large");
+    join.first = int(blocks);
+    const int64_t more = join.db ? div_up(join.N, kJoinColumns) : 0;
+    hipLaunchKernelGGL(linear_finish<E>, dim3(unsigned(blocks + more)), dim3(256), 0, s, g.part, plan.splits, g.M, g.N, g.epi,
+                       join);
     GD_LAUNCH_CHECK("linear_finish");
   }
   return GD_OK;
@@ -1458,6 +1473,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     rz = {reinterpret_cast<uint16_t*>(ws), n8, n8};
     ws += align256(size_t(M) * n8 * 2);
   }
+  Join join = {};
   const Rows rw = dx ? rows_of(w, ldw, K) : Rows();
   const Epi to_dx = dx ? plain_epi(dx, dx_dtype == GD_F32, lddx) : Epi();
   const bool together = dx && act != kNone && dy_dtype != GD_F32 && aligned(dy, 16) && lddy % 8 == 0 && aligned(z, 16) &&
@@ -1489,11 +1505,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     else
       hipLaunchKernelGGL((linear_dz_dx<E, 4>), dim3(blocks), dim3(256), 0, s, a);
     GD_LAUNCH_CHECK("linear_dz_dx");
-    if (db) {
-      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(kSumThreads), 0, s, a.sums, blocks, N, db,
-                         int(param_dtype == GD_F32));
-      GD_LAUNCH_CHECK("linear_colsum");
-    }
+    if (db) join = {a.sums, db, blocks, N, int(param_dtype == GD_F32), 0};
   } else if (db || (make && (dx || dw))) {
     const DactPlan d = dact_plan(M, N);
     Dact a = {};
@@ -1517,11 +1529,7 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     }
     hipLaunchKernelGGL(linear_dact<E>, dim3(d.blocks, d.slabs), dim3(256), 0, s, a);
     GD_LAUNCH_CHECK("linear_dact");
-    if (db) {
-      hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, 32))), dim3(kSumThreads), 0, s, a.sums, d.blocks, N,
-                         db, int(param_dtype == GD_F32));
-      GD_LAUNCH_CHECK("linear_colsum");
-    }
+    if (db) join = {a.sums, db, d.blocks, N, int(param_dtype == GD_F32), 0};
   }
   if (dx && !together) {
     Gemm g = {};
@@ -1552,7 +1560,13 @@ gd_status backward(int act, const void* dy, int dy_dtype, int64_t lddy, const vo
     g.M = N;
     g.N = K;
     g.epi = plain_epi(dw, param_dtype == GD_F32, K);
-    GD_TRY((product<E, true, true>(plan_of(N, K, M), g, ws, s)));
+    const Plan p = plan_of(N, K, M);
+    GD_TRY((product<E, true, true>(p, g, ws, s, join)));
+    if (p.splits > 1) return GD_OK;  // (with the column sums)
+  }
+  if (join.db) {
+    hipLaunchKernelGGL(linear_colsum<E>, dim3(unsigned(div_up(N, kJoinColumns))), dim3(256), 0, s, join);
+    GD_LAUNCH_CHECK("linear_colsum");
   }
   return GD_OK;
 }
