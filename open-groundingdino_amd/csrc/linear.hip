@@ -50,6 +50,7 @@ typedef _Float16 gd_f16x8 __attribute__((ext_vector_type(8)));
 
 #ifndef GD_STORE_NT
 #define GD_STORE_NT(value, to) __builtin_nontemporal_store(value, to)
+#define GD_LOAD_NT(from) __builtin_nontemporal_load(from)
 #endif
 
 // the two 16-bit types
@@ -168,15 +169,26 @@ __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
   }
 }
 
+// 16 bytes of an input that is read once: it leaves the memory-side cache to what is read again (the layer 44446 x 256 ->
+// 2048 with its gradients 287 us with plain loads of dy and z, 264 with these, since dz is there when dW reads it;
+// with the slope as a kernel of its own 344 and 282)
+__device__ __forceinline__ uint4 ld_once(const void* p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 u = GD_LOAD_NT(static_cast<const u32x4*>(p));
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+
 // ---- 8 consecutive 16-bit or fp32 values, the first `left` of them valid ------
-template <typename E>
+// ONCE: see ld_once
+template <typename E, bool ONCE = false>
 __device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool vec, int left, float v[8]) {
   if (f32) {
     const float* q = static_cast<const float*>(p) + at;
     if (vec && left >= 8) {
-      const float4 a = reinterpret_cast<const float4*>(q)[0], b = reinterpret_cast<const float4*>(q)[1];
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      const uint4* const u = reinterpret_cast<const uint4*>(q);
+      const uint4 a = ONCE ? ld_once(u) : u[0], b = ONCE ? ld_once(u + 1) : u[1];
+      v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+      v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = j < left ? q[j] : 0.f;
@@ -189,7 +201,7 @@ __device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool ve
     uint16_t h[8];
   } w;
   if (vec && left >= 8) {
-    w.u = *reinterpret_cast<const uint4*>(q);
+    w.u = ONCE ? ld_once(q) : *reinterpret_cast<const uint4*>(q);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) w.h[j] = j < left ? q[j] : uint16_t(0);
@@ -1084,8 +1096,8 @@ __global__ void __launch_bounds__(256) linear_dact(const Dact p) {
 #pragma unroll
       for (int h = 0; h < kRowsAhead; ++h) {
         const int64_t row = m + h * rows < end ? m + h * rows : end - 1;
-        ld8<E>(p.dy, row * p.lddy + n, p.dy_f32, p.dy_vec, left, d[h]);
-        if (p.z) ld8<E>(p.z, row * p.ldz + n, false, p.z_vec, left, z[h]);
+        ld8<E, true>(p.dy, row * p.lddy + n, p.dy_f32, p.dy_vec, left, d[h]);
+        if (p.z) ld8<E, true>(p.z, row * p.ldz + n, false, p.z_vec, left, z[h]);
       }
 #pragma unroll
       for (int h = 0; h < kRowsAhead; ++h) {
@@ -1148,13 +1160,14 @@ __global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
     dy_at[h] = (uint32_t(r) * uint32_t(p.lddy) + 8 * ch) * 2;
     z_at[h] = (uint32_t(r) * uint32_t(p.ldz) + 8 * ch) * 2;
   }
-  uint16_t* dz = p.dz + int64_t(m0 + row) * p.lddz + 8 * ch;
+  uint16_t* dz = p.dz + int64_t(m0) * p.lddz;
+  const uint32_t dz_at = uint32_t(row) * uint32_t(p.lddz) + 8 * ch;
   uint4 dy_of[kPieces], z_of[kPieces];
   auto ask = [&]() {
 #pragma unroll
     for (int h = 0; h < kPieces; ++h) {
-      dy_of[h] = *reinterpret_cast<const uint4*>(dy + dy_at[h]);
-      z_of[h] = *reinterpret_cast<const uint4*>(z + z_at[h]);
+      dy_of[h] = ld_once(dy + dy_at[h]);
+      z_of[h] = ld_once(z + z_at[h]);
     }
     dy += 2 * kR;
     z += 2 * kR;
@@ -1191,7 +1204,7 @@ __global__ void __launch_bounds__(256, 3) linear_dz_dx(const DzDx p) {
         if (in) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) sum[j] += d[j];
-          if (p.dz) *reinterpret_cast<uint4*>(dz + 32 * h * p.lddz) = u;
+          if (p.dz) *reinterpret_cast<uint4*>(dz + 32 * h * p.lddz + dz_at) = u;
         }
       }
     };
@@ -1301,7 +1314,7 @@ int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 //   128 x 128  the same 485 us in 8 rounds; 8400 x 1536 x 384 in one, 198 workgroups: 20 us
 //   64 x 64    900 x 256 x 256 in one round of 60: 4.6 us (by 128s 7.1)
 // Parts of a split sum are written and read once more, in fp32 at about 6 TB/s (they stay near), by a further launch.
-// Over 72 products of this detector's sizes the choice is 0.6 % off the best of the three on average, 10 % at most.
+// Over 72 products of this detector's sizes and wider ones the choice is 0.7 % off the best of the three on average, 14 % at most.
 struct Plan {
   int tile, splits, r_per_split;
   size_t bytes;
@@ -1413,8 +1426,8 @@ DactPlan dact_plan(int M, int N) {
 
 // Whether the backward of an activation and dx are one kernel (the rest of the conditions is about the pieces).  Its
 // workgroups take some 1.8 us per chunk whatever their number, so it pays for many rows, and where dz on its way
-// through memory costs more than its place in the caches: 44446 x 256 <- 2048 218 us and 261 apart (the whole
-// backward), 33400 x 192 <- 768 81 and 91; 16384 x 256 <- 1024 66 and 62, 8192 x 256 <- 2048 79 and 58.
+// through memory costs more than its place in the caches: 44446 x 256 <- 2048 193 us and 217 apart (the whole
+// backward), 33400 x 192 <- 768 84 and 94; 16384 x 256 <- 1024 66 and 65, 8192 x 256 <- 2048 79 and 62.
 bool dz_dx_fits(int M, int K, int N) {
   const int from = env_int("GD_LINEAR_TOGETHER", 0);  // (A/B: rows)
   return K <= 256 && (from > 0 ? M >= from : M >= 24576 && int64_t(M) * N >= 20000000);

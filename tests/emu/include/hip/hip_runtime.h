@@ -483,6 +483,7 @@ inline int __ffsll(long long v) { return __builtin_ffsll(v); }
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_sqrtf(x) sqrtf(x)
 #define GD_STORE_NT(value, to) (*(to) = (value))
+#define GD_LOAD_NT(from) (*(from))
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, cbsz, abid, blgp) ::gd_emu::mfma_16x16x32_f16((a), (b), (c))
 #define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) ::gd_emu::fdot2_bf16((a), (b), (c))
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) ::gd_emu::mfma_16x16x4_f32((a), (b), (c))
