@@ -339,7 +339,9 @@ gd_status adamw_launch(int tensors, const AdamLists& l, const AdamConst& c, hipS
     blocks = 0;
     return GD_OK;
   };
-  for (int i = 0; i < tensors; ++i) {
+  // from the last tensor on: the norm, which goes from the first, has left the last gradients in the memory-side cache (400 M
+  // masters with clipping 1248 us in the lists' order, 1225 in this one)
+  for (int i = tensors - 1; i >= 0; --i) {
     for (int64_t off = 0; off < l.n[i]; off += kOpPiece) {
       const uint32_t n = uint32_t(l.n[i] - off < int64_t(kOpPiece) ? l.n[i] - off : int64_t(kOpPiece));
       const int e = t.entries++;
