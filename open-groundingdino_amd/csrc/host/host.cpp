@@ -127,7 +127,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                         const Tensor& wc, const std::optional<Tensor>& bc, int64_t act) {
     const Tensor r = residual ? rows_of(*residual) : Tensor();
     const bool wants = x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad());
-    // of a ReLU without a residual, y itself tells where z > 0
+    // of a ReLU without a residual, y itself tells where z <= 0
     const bool by_y = act == 1 && !residual;
     const Tensor x2 = rows_of(xc);
     const Forward f = linear_forward(x2, wc, bc ? *bc : Tensor(), int(act), r, wants && act != 0 && !by_y,

@@ -14,7 +14,7 @@
 // matrix-core registers; bias, activation and residual are applied to them in
 // fp32 and the result is rounded once.  The backward rounds dz to 16 bits, as the
 // matrix instructions take it, and needs act'(z): the forward writes z rounded to
-// 16 bits beside y (for ReLU without a residual y itself tells where z > 0).
+// 16 bits beside y (for ReLU without a residual y itself tells where z <= 0).
 //
 // Where the output has too few tiles to fill 256 CUs the sum over r is split: the
 // parts go to a workspace in fp32 and a finishing kernel adds them in a fixed
@@ -141,7 +141,7 @@ __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
   switch (act) {
     case kRelu:
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[j] = z[j] > 0.f ? d[j] : 0.f;
+      for (int j = 0; j < 8; ++j) d[j] = z[j] <= 0.f ? 0.f : d[j];  // (at NaN, as the forward keeps it, dy goes on)
       break;
     case kGelu:
 #pragma unroll

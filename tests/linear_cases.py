@@ -135,3 +135,24 @@ def check_around(device, m=333, k=136, n=192, pad=24):
         assert (ws[nbytes:] == 7).all()
         grads = inside(dx, m, k), inside(dw, n, k), inside(db, 1, n)[0], None
         check(x, w, b, "gelu", r, inside(y, m, n), dy, grads)
+
+
+def check_relu_at_nan(device, residual=None, m=70, k=24, n=64):
+    """A row of NaN, and an infinite one: ReLU's gradient is dy wherever z is not below or at zero, NaN among it."""
+    from gdino_amd.linear import linear_act
+    x, w, b, r, dy = inputs(m, k, n, torch.bfloat16, True, residual, seed=9, device=device)
+    bad = [3, m - 1]
+    with torch.no_grad():
+        x[3, 5], x[m - 1, 0] = float("nan"), float("inf")
+    y = linear_act(x, w, b, "relu", r)
+    assert torch.isnan(y[3]).all()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x64, w64, b64, d = (t.detach().cpu().double() for t in (x, w, b, dy))
+    z = x64 @ w64.t() + b64
+    near_zero = z.abs() <= (k + 2) * U * (x64.abs() @ w64.abs().t() + b64.abs())  # (its sign may go either way)
+    near_zero[bad] = False
+    dz = torch.where(z <= 0, torch.zeros_like(d), d)
+    slack = torch.where(near_zero, d.abs(), torch.zeros_like(d)) + half_step(x.dtype) * dz.abs()
+    near(dx, dz @ w64, slack @ w64.abs() + (n + 2) * U * (dz.abs() @ w64.abs()))
+    near(db, dz.sum(0), slack.sum(0) + (m + 2) * U * dz.abs().sum(0))
+    assert torch.isnan(dw[:, 5]).all() and not torch.isfinite(dw[z[m - 1].to(device) > 0, 0]).any()

@@ -279,3 +279,10 @@ def test_swin_mlp_runs_on_it(emulated, monkeypatch):
     size = (net.fc1(x).abs() + 1) @ net.fc2.weight.abs().t() + net.fc2.bias.abs()
     assert ((got - want).abs() <= 4 * lc.half_step(BF) * size).all()
     assert net(x.double().float()).dtype == F32  # without autocast: the plain composition
+
+
+@pytest.mark.parametrize("together", ["1", "1000000000"])
+@pytest.mark.parametrize("residual", [None, BF])
+def test_relu_gradient_at_nan(emulated, monkeypatch, together, residual):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_relu_at_nan("cpu", residual)

@@ -244,3 +244,10 @@ def test_train_step_in_a_graph():
     for a, b in zip(got, want):
         for s, t in zip(a, b):
             assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize("together", ["1", "1000000000"])
+@pytest.mark.parametrize("residual", [None, BF])
+def test_relu_gradient_at_nan(monkeypatch, together, residual):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_relu_at_nan("cuda", residual, m=1000, k=136, n=192)
