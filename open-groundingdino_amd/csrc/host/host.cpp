@@ -75,7 +75,11 @@ void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 // t as [rows, features] with the features contiguous
 Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  return r.stride(1) == 1 && r.stride(0) >= r.size(1) ? r : r.contiguous();
+  const int64_t cols = r.size(1), pitch = r.stride(0);
+  const bool dense = r.stride(1) == 1 || cols == 1;
+  // (a single row's pitch may be anything, and contiguous() leaves it)
+  if (dense && pitch < cols && r.size(0) == 1) return r.as_strided({1, cols}, {cols, 1});
+  return dense && pitch >= cols ? r : r.contiguous();
 }
 
 struct Forward {

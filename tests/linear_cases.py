@@ -156,3 +156,25 @@ def check_relu_at_nan(device, residual=None, m=70, k=24, n=64):
     near(dx, dz @ w64, slack @ w64.abs() + (n + 2) * U * (dz.abs() @ w64.abs()))
     near(db, dz.sum(0), slack.sum(0) + (m + 2) * U * dz.abs().sum(0))
     assert torch.isnan(dw[:, 5]).all() and not torch.isfinite(dw[z[m - 1].to(device) > 0, 0]).any()
+
+
+def one_row(t, strides):
+    """The first row of t as a [1, n] view whose rows are `strides[0]` apart (and its values `strides[1]`)."""
+    return t.detach().as_strided((1, t.shape[1]), strides)
+
+
+def check_one_row(device, m, n, strides, k=24):
+    """x, W, residual and dy of one row, whose pitch says nothing: shorter than the row, or zero."""
+    from gdino_amd.linear import linear_act
+    x, w, b, r, dy = inputs(m, k, n, torch.bfloat16, True, torch.bfloat16, seed=12, device=device, grad=False)
+    if m == 1:
+        x, r, dy = (one_row(t, strides) for t in (x, r, dy))
+    if n == 1:
+        w = one_row(w, strides)
+        r, dy = (t.expand(m, 1) for t in (r[:1], dy[:1]))
+    x, w, b, r = (t.requires_grad_() for t in (x, w, b, r))
+    assert any(t.shape[0] == 1 and t.stride(0) < t.shape[1] for t in (x, w))
+    y = linear_act(x, w, b, "gelu", r)
+    with torch.no_grad():
+        assert torch.equal(linear_act(x, w, b, "gelu", r), y)
+    check(x, w, b, "gelu", r, y, dy, torch.autograd.grad(y, (x, w, b, r), dy))

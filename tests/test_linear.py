@@ -286,3 +286,14 @@ def test_swin_mlp_runs_on_it(emulated, monkeypatch):
 def test_relu_gradient_at_nan(emulated, monkeypatch, together, residual):
     monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
     lc.check_relu_at_nan("cpu", residual)
+
+
+@pytest.mark.parametrize("strides", [(1, 1), (0, 1), (0, 0)])
+@pytest.mark.parametrize("m,n", [(1, 16), (5, 1), (1, 1)])
+def test_rows_whose_pitch_says_nothing(emulated, m, n, strides):
+    lc.check_one_row("cpu", m, n, strides)
+    from gdino_amd.linear import linear_act
+    x, w, b, _, _ = lc.inputs(m, 24, n, BF, seed=1)
+    linear_act(x, w, b).sum().backward()  # (dy expanded from one value)
+    want = w.detach().double().sum(0).expand(m, 24)
+    lc.near(x.grad, want, (n + 2) * lc.U * w.detach().double().abs().sum(0).expand(m, 24))

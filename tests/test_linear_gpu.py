@@ -251,3 +251,9 @@ def test_train_step_in_a_graph():
 def test_relu_gradient_at_nan(monkeypatch, together, residual):
     monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
     lc.check_relu_at_nan("cuda", residual, m=1000, k=136, n=192)
+
+
+@pytest.mark.parametrize("strides", [(1, 1), (0, 1), (0, 0)])
+@pytest.mark.parametrize("m,n", [(1, 520), (300, 1), (1, 1)])
+def test_rows_whose_pitch_says_nothing(m, n, strides):
+    lc.check_one_row("cuda", m, n, strides, k=256)
