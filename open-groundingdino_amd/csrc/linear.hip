@@ -136,6 +136,13 @@ __device__ __forceinline__ void activate8(float v[8], int act) {
   }
 }
 
+// Where the smooth slopes are 0 and 1 in fp32, z is taken as +-128: an infinite z (in fp16 any beyond 65504, whose
+// layer may well be finite with an fp32 residual) would make them inf * 0.  NaN stays.
+__device__ __forceinline__ float slope_arg(float z) {
+  z = z > 128.f ? 128.f : z;
+  return z < -128.f ? -128.f : z;
+}
+
 // d[j] *= act'(z[j])
 __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
   switch (act) {
@@ -146,23 +153,24 @@ __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
     case kGelu:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
+        const float x = slope_arg(z[j]);
         float bell;
-        const float c = normal_cdf(z[j], &bell);
-        d[j] *= c + z[j] * bell * 0.39894228040143268f;
+        const float c = normal_cdf(x, &bell);
+        d[j] *= c + x * bell * 0.39894228040143268f;
       }
       break;
     case kGeluTanh:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float q = tanh_gate(z[j]);
-        d[j] *= q + 2.f * z[j] * q * (1.f - q) * kTanhC * (1.f + 3.f * kTanhA * z[j] * z[j]);
+        const float x = slope_arg(z[j]), q = tanh_gate(x);
+        d[j] *= q + 2.f * x * q * (1.f - q) * kTanhC * (1.f + 3.f * kTanhA * x * x);
       }
       break;
     case kSilu:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float q = sigmoid(z[j]);
-        d[j] *= q * (1.f + z[j] * (1.f - q));
+        const float x = slope_arg(z[j]), q = sigmoid(x);
+        d[j] *= q * (1.f + x * (1.f - q));
       }
       break;
     default: break;

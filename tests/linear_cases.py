@@ -178,3 +178,26 @@ def check_one_row(device, m, n, strides, k=24):
     with torch.no_grad():
         assert torch.equal(linear_act(x, w, b, "gelu", r), y)
     check(x, w, b, "gelu", r, y, dy, torch.autograd.grad(y, (x, w, b, r), dy))
+
+
+def check_far_from_zero(device, act, dtype, size, residual, m=130, k=128, n=192):
+    """z = +-size everywhere, beyond the type's range or its squares beyond fp32's: the slopes are 0 and 1, exactly."""
+    from gdino_amd.linear import linear_act
+    x, w, b, r, dy = inputs(m, k, n, dtype, True, residual, seed=13, device=device, grad=False)
+    root = size ** 0.5
+    x[:, 0] = torch.where(x[:, 0] > 0, root, -root)
+    w[:, 0] = root
+    x[:, 1:] = 0
+    dy *= 2.0 ** -12
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = linear_act(x, w, b, act, r)
+    if residual == torch.float32:
+        assert torch.isfinite(y).all()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    x64, w64 = x.detach().cpu().double(), w.detach().cpu().double()
+    dz = torch.where(x64[:, :1] > 0, dy.cpu().double(), torch.zeros(m, n).double())
+    e = half_step(dtype) * dz.abs() + (2.0 ** -25 if dtype == torch.float16 else 0)
+    near(dx, dz @ w64, e @ w64.abs() + (n + 2) * U * (dz.abs() @ w64.abs()))
+    near(dw, dz.t() @ x64, e.t() @ x64.abs() + (m + 2) * U * (dz.abs().t() @ x64.abs()))
+    near(db, dz.sum(0), (m + 2) * U * dz.abs().sum(0) + 2.0 ** -25)

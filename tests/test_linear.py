@@ -297,3 +297,13 @@ def test_rows_whose_pitch_says_nothing(emulated, m, n, strides):
     linear_act(x, w, b).sum().backward()  # (dy expanded from one value)
     want = w.detach().double().sum(0).expand(m, 24)
     lc.near(x.grad, want, (n + 2) * lc.U * w.detach().double().abs().sum(0).expand(m, 24))
+
+
+@pytest.mark.parametrize("tile,together", [("64", "1000000000"), ("128", "1000000000"), ("256", "1000000000"), ("128", "1")])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_far_from_zero(emulated, monkeypatch, act, tile, together):
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_far_from_zero("cpu", act, HF, 90000.0, F32)
+    lc.check_far_from_zero("cpu", act, HF, 90000.0, None)
+    lc.check_far_from_zero("cpu", act, BF, 1e22, None)

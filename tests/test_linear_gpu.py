@@ -257,3 +257,13 @@ def test_relu_gradient_at_nan(monkeypatch, together, residual):
 @pytest.mark.parametrize("m,n", [(1, 520), (300, 1), (1, 1)])
 def test_rows_whose_pitch_says_nothing(m, n, strides):
     lc.check_one_row("cuda", m, n, strides, k=256)
+
+
+@pytest.mark.parametrize("tile,together", [("64", "1000000000"), ("128", "1000000000"), ("256", "1000000000"), ("128", "1")])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_far_from_zero(monkeypatch, act, tile, together):
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_far_from_zero("cuda", act, HF, 90000.0, F32)
+    lc.check_far_from_zero("cuda", act, HF, 90000.0, None)
+    lc.check_far_from_zero("cuda", act, BF, 1e22, None)
