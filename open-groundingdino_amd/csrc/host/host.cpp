@@ -13,7 +13,9 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -70,6 +72,20 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// Why a call cannot be made here and now, or NULL.  The operators are calls, not operations that torch sees: what records
+// operations (torch.jit.trace, make_fx, torch.export) would keep the outputs' allocation and none of their values.
+const char* obstacle() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+      (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
+    return "it cannot be traced (its kernels are not torch operations)";
+  return nullptr;
+}
+void require_no_obstacle(const char* what) {
+  const char* const why = obstacle();
+  TORCH_CHECK(!why, what, ": ", why);
+}
 
 // ------------------------------------------------------------------ linear layer
 // t as [rows, features] with the features contiguous
@@ -191,6 +207,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 // they are
 Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, Tensor xc, Tensor wc,
                   Tensor bc, int act) {
+  require_no_obstacle("linear_act");
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.numel() > 0,
                     "linear_act: x ", x.sizes(), " and weight ", weight.sizes(), " do not match");
   const int64_t n = weight.size(0);
@@ -351,6 +368,7 @@ PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 PyObject* py_grad_norm(PyObject*, PyObject* list) {
   return guarded([&]() -> PyObject* {
+    require_no_obstacle("grad_norm");
     std::optional<at::Device> device;
     const List g = list_of("grad_norm", "gradients", list, {at::kFloat, at::kBFloat16}, &device, false, nullptr);
     TORCH_CHECK_VALUE(!g.held.empty(), "grad_norm: no tensors");
@@ -374,6 +392,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
     return nullptr;
   return guarded([&]() -> PyObject* {
     const char* what = "adamw_step";
+    require_no_obstacle(what);
     std::optional<at::Device> device;
     const List lp = list_of(what, "weights", p, {at::kFloat}, &device, true, nullptr);
     const auto* size = &lp.size;
@@ -422,8 +441,17 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
   });
 }
 
+PyObject* py_obstacle(PyObject*, PyObject*) {
+  return guarded([&]() -> PyObject* {
+    const char* const why = obstacle();
+    if (why) return PyUnicode_FromString(why);
+    Py_RETURN_NONE;
+  });
+}
+
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_O, "the library's entry points: {name: address}"},
+    {"obstacle", py_obstacle, METH_NOARGS, "obstacle(): why an operator cannot be called here and now, or None"},
     {"linear_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_act)), METH_FASTCALL,
      "linear_act(x, weight, bias, residual, x's, weight's and bias's casts or None, activation)"},
     {"grad_norm", py_grad_norm, METH_O, "grad_norm(gradients)"},

@@ -59,10 +59,11 @@ def _low(t, dt):
 
 
 def supported(x, weight) -> bool:
-    """Whether linear_act takes these (on the device, in 16 bits or to be cast to it by autocast)."""
+    """Whether linear_act takes these (on the device, in 16 bits or to be cast to it by autocast; not while traced)."""
     dt = _compute_dtype(x)
     return (_lib.enabled("linear") and _lib.on_device(x) and dt in DTYPES and x.dtype in DTYPES + (torch.float32,)
-            and (weight.dtype == dt or weight.dtype == torch.float32) and (x.dtype == dt or x.dtype == torch.float32))
+            and (weight.dtype == dt or weight.dtype == torch.float32) and (x.dtype == dt or x.dtype == torch.float32)
+            and _lib.host().obstacle() is None)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias=None, activation: str = "none", residual=None) -> torch.Tensor:

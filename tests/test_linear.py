@@ -307,3 +307,41 @@ def test_slopes_far_from_zero(emulated, monkeypatch, act, tile, together):
     lc.check_far_from_zero("cpu", act, HF, 90000.0, F32)
     lc.check_far_from_zero("cpu", act, HF, 90000.0, None)
     lc.check_far_from_zero("cpu", act, BF, 1e22, None)
+
+
+@pytest.mark.parametrize("how", ["jit", "real", "fake", "pre_dispatch"])
+def test_tracing_is_refused_and_composed(emulated, monkeypatch, how):
+    """A trace would record the output's allocation without its values: the call refuses, the block and the
+    dispatched layer are traced as their library composition."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from gdino_amd import castcache, kernels, linear, optim
+    from models.GroundingDINO.backbone.swin_transformer import Mlp
+    castcache.clear()
+
+    def trace(f, *args):
+        if how == "jit":
+            return torch.jit.trace(f, args, check_trace=False)
+        return make_fx(f, tracing_mode="fake" if how == "fake" else "real", pre_dispatch=how == "pre_dispatch")(*args)
+
+    x, w, b, _, _ = lc.inputs(6, 24, 16, BF, grad=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        trace(lambda t, w, b: linear.linear_act(t, w, b, "relu"), x, w, b)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        trace(lambda t: optim.grad_norm([t]), torch.ones(5))
+
+    def update(t):
+        optim.adamw_step([t], [t + 1], [t * 0], [t * 0], 1, lr=1e-3)
+        return t
+
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        trace(update, torch.ones(5))
+    other = torch.randn(6, 24).to(BF)
+    f = trace(lambda t, w, b: kernels.linear_act(t, w, b, "gelu"), x, w, b)
+    assert torch.equal(f(other, w, b), linear._linear_act_torch(other, w, b, "gelu"))
+    if how == "fake":  # (a module's weights are not fake tensors)
+        return
+    net = Mlp(24, 40).to(BF).eval()
+    monkeypatch.setattr(linear, "FUSED_MLP", True)
+    f, want = trace(net, x), net(other)
+    monkeypatch.setattr(linear, "FUSED_MLP", False)
+    assert torch.equal(f(other), net(other)) and torch.equal(net(other).isfinite(), want.isfinite())
