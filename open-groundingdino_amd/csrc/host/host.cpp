@@ -14,6 +14,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -73,17 +74,23 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
-// Why a call cannot be made here and now, or NULL.  The operators are calls, not operations that torch sees: what records
-// operations (torch.jit.trace, make_fx, torch.export) would keep the outputs' allocation and none of their values.
-const char* obstacle() {
+// Why a call with these tensors cannot be made here and now, or NULL.  The operators are calls, not operations that torch
+// sees: what records operations (torch.jit.trace, make_fx, torch.export) would keep the outputs' allocation and none
+// of their values, and a dual tensor's tangent would be lost.
+const char* obstacle(std::initializer_list<const Tensor*> tensors) {
   using Modes = c10::impl::TorchDispatchModeTLS;
   if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
       (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
     return "it cannot be traced (its kernels are not torch operations)";
+  const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    if (forward_mode && t->_fw_grad(0).defined()) return "it has no forward-mode derivatives";
+  }
   return nullptr;
 }
-void require_no_obstacle(const char* what) {
-  const char* const why = obstacle();
+void require_no_obstacle(const char* what, std::initializer_list<const Tensor*> tensors = {}) {
+  const char* const why = obstacle(tensors);
   TORCH_CHECK(!why, what, ": ", why);
 }
 
@@ -207,7 +214,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 // they are
 Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, Tensor xc, Tensor wc,
                   Tensor bc, int act) {
-  require_no_obstacle("linear_act");
+  require_no_obstacle("linear_act", {&x, &weight, &bias, &residual});
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && weight.size(1) == x.size(-1) && weight.numel() > 0,
                     "linear_act: x ", x.sizes(), " and weight ", weight.sizes(), " do not match");
   const int64_t n = weight.size(0);
@@ -441,9 +448,13 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
   });
 }
 
-PyObject* py_obstacle(PyObject*, PyObject*) {
+PyObject* py_obstacle(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    const char* const why = obstacle();
+    const char* why = obstacle({});
+    for (Py_ssize_t i = 0; i < n && !why; ++i) {
+      const Tensor t = tensor_of(args[i]);
+      why = obstacle({&t});
+    }
     if (why) return PyUnicode_FromString(why);
     Py_RETURN_NONE;
   });
@@ -451,7 +462,8 @@ PyObject* py_obstacle(PyObject*, PyObject*) {
 
 PyMethodDef methods[] = {
     {"bind", py_bind, METH_O, "the library's entry points: {name: address}"},
-    {"obstacle", py_obstacle, METH_NOARGS, "obstacle(): why an operator cannot be called here and now, or None"},
+    {"obstacle", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_obstacle)), METH_FASTCALL,
+     "obstacle(tensor or None, ...): why an operator cannot be called with these here and now, or None"},
     {"linear_act", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_linear_act)), METH_FASTCALL,
      "linear_act(x, weight, bias, residual, x's, weight's and bias's casts or None, activation)"},
     {"grad_norm", py_grad_norm, METH_O, "grad_norm(gradients)"},

@@ -58,12 +58,13 @@ def _low(t, dt):
     return t.to(dt)
 
 
-def supported(x, weight) -> bool:
-    """Whether linear_act takes these (on the device, in 16 bits or to be cast to it by autocast; not while traced)."""
+def supported(x, weight, bias=None, residual=None) -> bool:
+    """Whether linear_act takes these (on the device, in 16 bits or to be cast to it by autocast; not while traced, no
+    dual tensors of forward-mode derivatives)."""
     dt = _compute_dtype(x)
     return (_lib.enabled("linear") and _lib.on_device(x) and dt in DTYPES and x.dtype in DTYPES + (torch.float32,)
             and (weight.dtype == dt or weight.dtype == torch.float32) and (x.dtype == dt or x.dtype == torch.float32)
-            and _lib.host().obstacle() is None)
+            and _lib.host().obstacle(x, weight, bias, residual) is None)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias=None, activation: str = "none", residual=None) -> torch.Tensor:
@@ -98,6 +99,11 @@ def mlp(x, fc1: torch.nn.Linear, fc2: torch.nn.Linear, activation: str = "gelu",
     return linear_act(h, fc2.weight, fc2.bias)
 
 
+def mlp_supported(x, fc1: torch.nn.Linear, fc2: torch.nn.Linear) -> bool:
+    """Whether mlp takes these (fc2's input has x's type or autocast's)."""
+    return supported(x, fc1.weight, fc1.bias) and supported(x, fc2.weight, fc2.bias)
+
+
 def _linear_act_torch(x, weight, bias=None, activation="none", residual=None):
     """The composition of library kernels."""
     y = F.linear(x, weight, bias)
@@ -111,7 +117,7 @@ def _linear_act_torch(x, weight, bias=None, activation="none", residual=None):
 
 
 def _linear_act_hip(x, weight, bias=None, activation="none", residual=None):
-    if supported(x, weight):
+    if supported(x, weight, bias, residual):
         return linear_act(x, weight, bias, activation, residual)
     return _linear_act_torch(x, weight, bias, activation, residual)
 

@@ -38,7 +38,7 @@ class Mlp(nn.Module):
         self.drop = nn.Dropout(drop)
 
     def forward(self, x):
-        if linear.FUSED_MLP and type(self.act) is nn.GELU and linear.supported(x, self.fc1.weight):
+        if linear.FUSED_MLP and type(self.act) is nn.GELU and linear.mlp_supported(x, self.fc1, self.fc2):
             return self.drop(linear.mlp(x, self.fc1, self.fc2, "gelu" if self.act.approximate == "none" else "gelu_tanh",
                                         self.drop))
         return self.drop(self.fc2(self.drop(self.act(self.fc1(x)))))

@@ -345,3 +345,28 @@ def test_tracing_is_refused_and_composed(emulated, monkeypatch, how):
     f, want = trace(net, x), net(other)
     monkeypatch.setattr(linear, "FUSED_MLP", False)
     assert torch.equal(f(other), net(other)) and torch.equal(net(other).isfinite(), want.isfinite())
+
+
+def test_forward_mode_is_refused_and_composed(emulated, monkeypatch):
+    """A dual tensor's tangent is not dropped: the call refuses, the dispatched layer and the block compose."""
+    import torch.autograd.forward_ad as fwd
+    from gdino_amd import kernels, linear
+    from models.GroundingDINO.backbone.swin_transformer import Mlp
+    x, w, b, r, t = lc.inputs(6, 24, 16, BF, True, BF, grad=False)
+    tangents = [torch.randn(a.shape, generator=torch.Generator().manual_seed(i)).to(BF) for i, a in enumerate((x, w, b, r))]
+    with fwd.dual_level():
+        for i in range(4):
+            args = [x, w, b, r]
+            args[i] = fwd.make_dual(args[i], tangents[i])
+            for grad in (False, True):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    linear.linear_act(*args[:3], "gelu", args[3])
+            got = fwd.unpack_dual(kernels.linear_act(*args[:3], "gelu", args[3]))
+            want = fwd.unpack_dual(linear._linear_act_torch(*args[:3], "gelu", args[3]))
+            assert want.tangent.any() and torch.equal(got.tangent, want.tangent) and torch.equal(got.primal, want.primal)
+        with fwd._set_fwd_grad_enabled(False):
+            assert torch.equal(linear.linear_act(*args[:3], "gelu", args[3]), linear.linear_act(x, w, b, "gelu", r))
+    monkeypatch.setattr(linear, "FUSED_MLP", True)
+    net = Mlp(24, 40).to(BF).eval()
+    with fwd.dual_level(), torch.no_grad():
+        assert fwd.unpack_dual(net(fwd.make_dual(x, tangents[0]))).tangent is not None
