@@ -74,9 +74,18 @@ Tensor workspace(size_t bytes, const Tensor& like) {
 const void* data(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* mut(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+constexpr const char* kWrapped = "it takes plain tensors, no wrappers around them (vmap, torch.func, FakeTensor, DTensor)";
+bool wrapped(const Tensor& t) {
+  using c10::DispatchKey;
+  static const c10::DispatchKeySet keys({DispatchKey::Python, DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
+                                         DispatchKey::Batched, DispatchKey::Functionalize});
+  return t.key_set().has_any(keys);
+}
+
 // Why a call with these tensors cannot be made here and now, or NULL.  The operators are calls, not operations that torch
 // sees: what records operations (torch.jit.trace, make_fx, torch.export) would keep the outputs' allocation and none
-// of their values, and a dual tensor's tangent would be lost.
+// of their values, and a dual tensor's tangent would be lost.  A wrapper (FakeTensor, DTensor, what vmap and torch.func
+// hand on) has no memory to be read.
 const char* obstacle(std::initializer_list<const Tensor*> tensors) {
   using Modes = c10::impl::TorchDispatchModeTLS;
   if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
@@ -85,6 +94,7 @@ const char* obstacle(std::initializer_list<const Tensor*> tensors) {
   const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : tensors) {
     if (!t->defined()) continue;
+    if (wrapped(*t)) return kWrapped;
     if (forward_mode && t->_fw_grad(0).defined()) return "it has no forward-mode derivatives";
   }
   return nullptr;
@@ -291,6 +301,7 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
     PyObject* o = tuple ? PyTuple_GET_ITEM(list, i) : PyList_GET_ITEM(list, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": ", name, " ", i, " is not a tensor but ", Py_TYPE(o)->tp_name);
     const Tensor& t = THPVariable_Unpack(o);
+    TORCH_CHECK_TYPE(!wrapped(t), what, ": ", name, " ", i, ": ", kWrapped);
     TORCH_CHECK(t.layout() == at::kStrided && t.is_contiguous(), name, " tensors have to be contiguous (", what, ")");
     TORCH_CHECK_TYPE((t.scalar_type() == types.a || t.scalar_type() == types.b) && (i == 0 || t.scalar_type() == out.held[0].scalar_type()),
                      "gdino_amd ", what, ": unsupported or mixed dtypes of ", name);

@@ -370,3 +370,26 @@ def test_forward_mode_is_refused_and_composed(emulated, monkeypatch):
     net = Mlp(24, 40).to(BF).eval()
     with fwd.dual_level(), torch.no_grad():
         assert fwd.unpack_dual(net(fwd.make_dual(x, tangents[0]))).tangent is not None
+
+
+def test_wrappers_are_refused_and_composed(emulated):
+    """vmap, torch.func's transforms and FakeTensor hand on tensors without memory: a reason, or the composition."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from gdino_amd import kernels, linear, optim
+    x, w, b, _, _ = lc.inputs(6, 24, 16, BF, grad=False)
+
+    def loss(layer):
+        return lambda t: layer(t, w, b, "gelu").float().square().sum()
+
+    for transform, arg in ((torch.vmap, x[None]), (torch.func.grad, x), (lambda f: torch.func.vmap(torch.func.grad(f)), x[None])):
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            transform(loss(linear.linear_act))(arg)
+        want = transform(loss(linear._linear_act_torch))(arg)
+        assert torch.equal(transform(loss(kernels.linear_act))(arg), want)
+    with FakeTensorMode() as mode:
+        fx, fw, fb = (mode.from_tensor(t) for t in (x, w, b))
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            linear.linear_act(fx, fw, fb)
+        assert kernels.linear_act(fx, fw, fb).shape == (6, 16)
+        with pytest.raises(TypeError, match="gradients 0: .* plain tensors"):
+            optim.grad_norm([fx])
