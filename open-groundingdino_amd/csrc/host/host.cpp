@@ -107,7 +107,7 @@ void require_no_obstacle(const char* what, std::initializer_list<const Tensor*> 
 // ------------------------------------------------------------------ linear layer
 // t as [rows, features] with the features contiguous
 Tensor rows_of(const Tensor& t) {
-  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  Tensor r = (t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})).resolve_neg();
   const int64_t cols = r.size(1), pitch = r.stride(0);
   const bool dense = r.stride(1) == 1 || cols == 1;
   // (a single row's pitch may be anything, and contiguous() leaves it)
@@ -258,13 +258,13 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias, con
     {
       const at::AutoGradMode off(false);
       wc = rows_of(wc);
-      if (bc.defined()) bc = bc.contiguous();
+      if (bc.defined()) bc = bc.resolve_neg().contiguous();
     }
     return LinearFunction::apply(x, weight, opt(bias), opt(residual), xc.detach(), wc.detach(),
                                  bc.defined() ? std::optional<Tensor>(bc.detach()) : std::nullopt, int64_t(act));
   }
   const at::AutoGradMode off(false);
-  return linear_forward(rows_of(xc), rows_of(wc), bc.defined() ? bc.contiguous() : bc, act,
+  return linear_forward(rows_of(xc), rows_of(wc), bc.defined() ? bc.resolve_neg().contiguous() : bc, act,
                         residual.defined() ? rows_of(residual) : residual, false, x.sizes())
       .y;
 }
@@ -302,6 +302,7 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": ", name, " ", i, " is not a tensor but ", Py_TYPE(o)->tp_name);
     const Tensor& t = THPVariable_Unpack(o);
     TORCH_CHECK_TYPE(!wrapped(t), what, ": ", name, " ", i, ": ", kWrapped);
+    TORCH_CHECK_VALUE(!t.is_neg(), what, ": ", name, " ", i, " is a negated view; resolve_neg() first");
     TORCH_CHECK(t.layout() == at::kStrided && t.is_contiguous(), name, " tensors have to be contiguous (", what, ")");
     TORCH_CHECK_TYPE((t.scalar_type() == types.a || t.scalar_type() == types.b) && (i == 0 || t.scalar_type() == out.held[0].scalar_type()),
                      "gdino_amd ", what, ": unsupported or mixed dtypes of ", name);

@@ -393,3 +393,15 @@ def test_wrappers_are_refused_and_composed(emulated):
         assert kernels.linear_act(fx, fw, fb).shape == (6, 16)
         with pytest.raises(TypeError, match="gradients 0: .* plain tensors"):
             optim.grad_norm([fx])
+
+
+def test_negated_views(emulated):
+    """A view that stands for its memory's negative (the imaginary part of a conjugate) is read as the value it is."""
+    from gdino_amd.linear import linear_act
+    x, w, b, r, dy = lc.inputs(6, 24, 16, BF, True, BF, grad=False)
+    want_y, want = lc.run(*(t.clone().requires_grad_() for t in (x, w, b)), "gelu", r.clone().requires_grad_(), dy)
+    nx, nw, nb, nr, ndy = (torch._neg_view(-t) for t in (x, w, b, r, dy))
+    assert nx.is_neg() and torch.equal(nx, x)
+    assert torch.equal(linear_act(nx, nw, nb, "gelu", nr), want_y)
+    y, got = lc.run(*(t.detach().requires_grad_() for t in (nx, nw, nb)), "gelu", nr.detach().requires_grad_(), ndy)
+    assert torch.equal(y, want_y) and all(torch.equal(a, c) for a, c in zip(got, want))

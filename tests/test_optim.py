@@ -288,3 +288,15 @@ def test_train_step_uses_it(emulated):
     train.clip_and_step(net.parameters(), opt, 0.1)
     assert all(torch.equal(p.grad, k) for p, k in zip(net.parameters(), kept))
     assert all(p._version > v for p, v in zip(net.parameters(), versions)) and castcache._generation == generation + 1
+
+
+def test_negated_views_are_refused(emulated):
+    from gdino_amd import optim
+    p, g, m, v = oc.make([8])
+    for i in range(4):
+        lists = [p, g, m, v]
+        lists[i] = [torch._neg_view(lists[i][0])]
+        with pytest.raises(ValueError, match="negated view"):
+            optim.adamw_step(*lists, 1, **oc.HYPER)
+    with pytest.raises(ValueError, match="negated view"):
+        optim.grad_norm([torch._neg_view(g[0])])
