@@ -310,7 +310,8 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
     TORCH_CHECK(t.device() == **device, what, ": ", name, " are not all on the device of the first tensor");
     out.size[i] = t.numel();
     TORCH_CHECK_VALUE(!sizes || (*sizes)[i] == out.size[i], what, ": ", name, " and the weights differ in their numbers of elements");
-    out.at[i] = out.size[i] ? reinterpret_cast<uint64_t>(t.const_data_ptr()) : 0;
+    // (a tensor that is written stops sharing a lazy clone's memory first)
+    out.at[i] = out.size[i] ? reinterpret_cast<uint64_t>(written ? t.mutable_data_ptr() : t.const_data_ptr()) : 0;
     if (written && out.size[i]) spans.emplace_back(out.at[i], out.at[i] + uint64_t(out.size[i]) * t.element_size());
     out.held.push_back(t);
   }

@@ -300,3 +300,15 @@ def test_negated_views_are_refused(emulated):
             optim.adamw_step(*lists, 1, **oc.HYPER)
     with pytest.raises(ValueError, match="negated view"):
         optim.grad_norm([torch._neg_view(g[0])])
+
+
+def test_lazy_clones_are_written_apart(emulated):
+    """A copy-on-write clone gets memory of its own before the step writes it."""
+    from gdino_amd import optim
+    for i in (0, 2, 3):
+        lists = oc.make([40])
+        kept = lists[i][0].clone()
+        original = lists[i][0]
+        lists[i][0] = torch._lazy_clone(original)
+        optim.adamw_step(*lists, 1, **oc.HYPER)
+        assert torch.equal(original, kept) and not torch.equal(lists[i][0], kept)
