@@ -58,13 +58,25 @@ def _low(t, dt):
     return t.to(dt)
 
 
-def supported(x, weight, bias=None, residual=None) -> bool:
-    """Whether linear_act takes these (on the device, in 16 bits or to be cast to it by autocast; not while traced, no
-    dual tensors of forward-mode derivatives)."""
+def _takes_weights(x, k, weight, bias):
+    """Whether weight and bias belong to a product of k features in x's place and type."""
     dt = _compute_dtype(x)
-    return (_lib.enabled("linear") and _lib.on_device(x) and dt in DTYPES and x.dtype in DTYPES + (torch.float32,)
-            and (weight.dtype == dt or weight.dtype == torch.float32) and (x.dtype == dt or x.dtype == torch.float32)
-            and _lib.host().obstacle(x, weight, bias, residual) is None)
+    return (weight.dim() == 2 and weight.shape[1] == k and 0 < k <= 1 << 22 and 0 < weight.shape[0] <= 1 << 22
+            and weight.dtype in (dt, torch.float32) and weight.device == x.device
+            and (bias is None or (bias.dtype == weight.dtype and bias.shape == weight.shape[:1] and bias.device == x.device)))
+
+
+def supported(x, weight, bias=None, residual=None) -> bool:
+    """Whether linear_act takes these: on the device, in 16 bits or to be cast to it by autocast, the bias of the
+    weight's type, a residual of y's shape; not while traced, no dual tensors of forward-mode derivatives, no wrappers."""
+    dt = _compute_dtype(x)
+    if not (_lib.enabled("linear") and _lib.on_device(x) and dt in DTYPES and x.dtype in (dt, torch.float32)
+            and x.dim() >= 1 and _takes_weights(x, x.shape[-1], weight, bias) and x.numel() // x.shape[-1] <= 1 << 30):
+        return False
+    if residual is not None and (residual.dtype not in (dt, torch.float32) or residual.device != x.device
+                                 or residual.shape != x.shape[:-1] + weight.shape[:1]):
+        return False
+    return _lib.host().obstacle(x, weight, bias, residual) is None
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias=None, activation: str = "none", residual=None) -> torch.Tensor:
@@ -100,8 +112,9 @@ def mlp(x, fc1: torch.nn.Linear, fc2: torch.nn.Linear, activation: str = "gelu",
 
 
 def mlp_supported(x, fc1: torch.nn.Linear, fc2: torch.nn.Linear) -> bool:
-    """Whether mlp takes these (fc2's input has x's type or autocast's)."""
-    return supported(x, fc1.weight, fc1.bias) and supported(x, fc2.weight, fc2.bias)
+    """Whether mlp takes these."""
+    return (supported(x, fc1.weight, fc1.bias) and _takes_weights(x, fc1.out_features, fc2.weight, fc2.bias)
+            and _lib.host().obstacle(fc2.weight, fc2.bias) is None)
 
 
 def _linear_act_torch(x, weight, bias=None, activation="none", residual=None):

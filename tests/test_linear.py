@@ -405,3 +405,34 @@ def test_negated_views(emulated):
     assert torch.equal(linear_act(nx, nw, nb, "gelu", nr), want_y)
     y, got = lc.run(*(t.detach().requires_grad_() for t in (nx, nw, nb)), "gelu", nr.detach().requires_grad_(), ndy)
     assert torch.equal(y, want_y) and all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_dispatch_composes_what_the_layer_does_not_take(emulated):
+    """What F.linear and an addition take: a bias of another type under autocast, a residual that is broadcast or in
+    64 bits, no features, a vector of weights, other types than autocast's."""
+    from gdino_amd import castcache, kernels, linear
+    castcache.clear()
+    x, w, b, r, _ = lc.inputs(6, 24, 16, BF, True, BF, grad=False)
+
+    def same(*args):
+        assert not linear.supported(*args)
+        got, want = kernels.linear_act(*args[:3], "gelu", *args[3:]), linear._linear_act_torch(*args[:3], "gelu", *args[3:])
+        assert got.dtype == want.dtype and torch.equal(got, want)
+
+    same(x, w, b, r[0])
+    same(x, w, b, r[:, :1])
+    same(x, w, b, r.double())
+    same(x, w, b, r.half())
+    same(x, w, b, torch.tensor(2.0))
+    same(x[:, :0], w[:, :0], b)
+    same(x, w[:0], b[:0])
+    same(x, w[0], None)
+    same(x.float(), w.float(), b.float())
+    with torch.autocast("cpu", dtype=BF):
+        same(x.float(), w.float(), b)
+        same(x, w, b.float())
+        same(x.half(), w, b)
+        same(x, w, b.half())
+    assert linear.supported(x, w, b, r) and linear.supported(x, w, b, r.float()) and linear.supported(x[0], w, b, r[0])
+    y = kernels.linear_act(x, w, b, "gelu", r)
+    assert torch.equal(y, linear.linear_act(x, w, b, "gelu", r))
