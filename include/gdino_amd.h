@@ -644,8 +644,8 @@ gd_status gd_linear_forward(int dtype, const void* x, int64_t ldx, const void* w
  * dz = dy * act'(z), dx[M, K] = dz W, dw[N, K] = dz^T x, db[N] = sum over rows of
  * dz (fp32 sums of unrounded dz; dz is rounded to `dtype` for the products).
  * dy: of `dtype` or fp32.  z as the forward wrote it, or of a ReLU without a
- * residual its y; unused without an activation.  x, W: as in the forward.  dx, dw, db:
- * NULL where not wanted; dx of dx_dtype, dw (contiguous) and db of param_dtype: `dtype` or fp32.
+ * residual its y; unused without an activation.  x (for dw only) and W (for dx only): as in
+ * the forward.  dx, dw, db: NULL where not wanted; dx of dx_dtype, dw (contiguous) and db of param_dtype: `dtype` or fp32.
  * M >= 1.  Both calls can be captured into a graph. */
 size_t gd_linear_backward_workspace_bytes(int M, int K, int N, int dx, int dw, int db);
 gd_status gd_linear_backward(int dtype, int act, const void* dy, int dy_dtype, int64_t lddy, const void* z, int64_t ldz,

@@ -169,10 +169,14 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const Tensor x2 = rows_of(xc);
     const Forward f = linear_forward(x2, wc, bc ? *bc : Tensor(), int(act), r, wants && act != 0 && !by_y,
                                      x.sizes());
-    ctx->save_for_backward({f.x, f.w, by_y ? f.y : f.z});
+    // x for W's gradient, W for x's, z or y for the slope
+    ctx->save_for_backward({weight.requires_grad() ? f.x : Tensor(), x.requires_grad() ? f.w : Tensor(),
+                            !wants || act == 0 ? Tensor() : by_y ? f.y : f.z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["x"] = x.sizes().vec();
-    ctx->saved_data["types"] = std::vector<int64_t>{int64_t(x.scalar_type()), int64_t(weight.scalar_type())};
+    ctx->saved_data["of"] = std::vector<int64_t>{x2.size(0), weight.size(0)};
+    ctx->saved_data["types"] =
+        std::vector<int64_t>{int64_t(x.scalar_type()), int64_t(weight.scalar_type()), int64_t(xc.scalar_type())};
     ctx->saved_data["given"] = std::vector<int64_t>{bias.has_value(), residual.has_value()};
     return f.y;
   }
@@ -190,9 +194,10 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const bool want_b = given[0] && ctx->needs_input_grad(2), want_r = given[1] && ctx->needs_input_grad(2 + given[0]);
     const auto shape = ctx->saved_data["x"].toIntVector();
-    const int64_t m = x.size(0), k = shape.back(), n = w.size(0);
+    const auto of = ctx->saved_data["of"].toIntVector();
+    const int64_t m = of[0], k = shape.back(), n = of[1];
     const auto xt = at::ScalarType(types[0]), wt = at::ScalarType(types[1]);
-    const auto like = x.options().requires_grad(false);
+    const auto like = dy.options().requires_grad(false);
     Tensor dx, dw, db;
     if (want_x) dx = at::empty({m, k}, like.dtype(xt));
     if (want_w) dw = at::empty({n, k}, like.dtype(wt));
@@ -204,13 +209,14 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       const Tensor g = rows_of(dy);
       Tensor z = saved[2];
       if (z.defined()) z = z.dim() == 2 ? z : z.reshape({m, -1});
-      const c10::DeviceGuard guard(x.device());
+      const c10::DeviceGuard guard(g.device());
       const size_t bytes = api.linear_backward_bytes(m, k, n, want_x, want_w, want_b);
-      const Tensor ws = workspace(bytes, x);
+      const Tensor ws = workspace(bytes, g);
+      const auto pitch = [](const Tensor& t) { return t.defined() ? t.stride(0) : 0; };
       run("gd_linear_backward",
-          api.linear_backward(code_of(x.scalar_type()), act, data(g), code_of(g.scalar_type()), g.stride(0), data(z),
-                              z.defined() ? z.stride(0) : 0, data(x), x.stride(0), data(w), w.stride(0), m, k, n, mut(dx),
-                              code_of(xt), k, mut(dw), mut(db), code_of(wt), 1, mut(ws), bytes, stream_of(x)));
+          api.linear_backward(code_of(at::ScalarType(types[2])), act, data(g), code_of(g.scalar_type()), g.stride(0), data(z),
+                              pitch(z), data(x), pitch(x), data(w), pitch(w), m, k, n, mut(dx), code_of(xt), k, mut(dw),
+                              mut(db), code_of(wt), 1, mut(ws), bytes, stream_of(g)));
     }
     if (want_x) out[0] = dx.view(shape);
     out[1] = dw;

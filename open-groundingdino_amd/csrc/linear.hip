@@ -1679,7 +1679,8 @@ extern "C" gd_status gd_linear_backward(int dtype, int act, const void* dy, int 
                                         gd_stream_t stream) {
   GD_TRY(check_shape(dtype, act, M, K, N));
   GD_REQUIRE(M > 0, "linear: gradients of no rows");
-  GD_REQUIRE(dy && x && w && lddy >= N && ldx >= K && ldw >= K && (!dx || lddx >= K), "linear: null pointer or short rows");
+  GD_REQUIRE(dy && lddy >= N && (!dw || (x && ldx >= K)) && (!dx || (w && ldw >= K && lddx >= K)),
+             "linear: null pointer or short rows");
   GD_REQUIRE(dy_dtype == dtype || dy_dtype == GD_F32, "linear: dy is fp32 or of the operands' type");
   GD_REQUIRE((dx_dtype == dtype || dx_dtype == GD_F32) && (param_dtype == dtype || param_dtype == GD_F32),
              "linear: gradients are fp32 or of the operands' type");

@@ -436,3 +436,26 @@ def test_dispatch_composes_what_the_layer_does_not_take(emulated):
     assert linear.supported(x, w, b, r) and linear.supported(x, w, b, r.float()) and linear.supported(x[0], w, b, r[0])
     y = kernels.linear_act(x, w, b, "gelu", r)
     assert torch.equal(y, linear.linear_act(x, w, b, "gelu", r))
+
+
+@pytest.mark.parametrize("act,residual", [("none", BF), ("relu", None), ("relu", F32), ("gelu", BF)])
+@pytest.mark.parametrize("k", [24, 17])
+def test_saved_tensors(emulated, act, residual, k):
+    """The backward keeps what its gradients need: x for W's, W for x's, z (or y) for an activation's slope."""
+    from gdino_amd.linear import linear_act
+    for which in range(1, 16):
+        x, w, b, r, dy = lc.inputs(9, k, 16, BF, True, residual, seed=5, grad=False)
+        leaves = [t for i, t in enumerate((x, w, b, r)) if which >> i & 1 and t is not None]
+        if not leaves:
+            continue
+        for t in leaves:
+            t.requires_grad_()
+        saved = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (saved.append(t.shape), t)[1], lambda t: t):
+            y = linear_act(x, w, b, act, r)
+        k8 = (k + 7) // 8 * 8
+        want = ([(9, k8)] if w.requires_grad else []) + ([(16, k8)] if x.requires_grad else [])
+        want += [(9, 16)] if act != "none" and (x.requires_grad or w.requires_grad or b.requires_grad) else []
+        assert saved == want, which
+        got = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, dy)))
+        lc.check(x, w, b, act, r, y, dy, [got.get(id(t)) for t in (x, w, b, r)])
