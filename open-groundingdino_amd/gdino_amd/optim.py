@@ -56,6 +56,14 @@ def _timed(name, tensors, factor, call):
     return out
 
 
+def _learning_rate(lr, device):
+    """(the tensor that the kernel reads, or None; the number).  A host tensor beside device weights is a number: it is
+    read now, and a captured step keeps it."""
+    if torch.is_tensor(lr) and (not lr.is_cpu or lr.device == device):
+        return lr, 0.0
+    return None, float(lr)
+
+
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2,
                exp_avg_scales=None, exp_avg_sq_scales=None, copies=None, total_norm=None, max_norm=0.0, seed=0) -> None:
     """One AdamW update, in place, of the fp32 tensors ``params``:
@@ -68,7 +76,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     ``exp_avg_scales`` and ``exp_avg_sq_scales`` (one byte per BLOCK elements, 2^(byte - 127)), m and sqrt(v) as
     e4m3 bytes (``adamw_state`` makes either).  step: t, counted from 1, or a
     list of one-element fp32 device tensors that hold it (they are read, not
-    advanced).  lr: a number or a one-element fp32 device tensor.  copies: bf16
+    advanced).  lr: a number (or a host tensor that holds it) or a one-element fp32 device tensor.  copies: bf16
     tensors that receive the new weights.  total_norm: ``grad_norm``'s result.
     seed: of the 8-bit moments' stochastic rounding.
 
@@ -87,10 +95,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     b1, b2 = betas
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0 and weight_decay >= 0.0):
         raise ValueError(f"{what}: betas {betas}, eps {eps}, weight_decay {weight_decay}")
-    lr_dev = None
-    if torch.is_tensor(lr) and (steps is not None or not lr.is_cpu):
-        lr_dev, lr = lr, 0.0
-    lr = float(lr)
+    lr_dev, lr = _learning_rate(lr, params[0].device if params else None)
     if not (lr >= 0.0 and math.isfinite(lr)):
         raise ValueError(f"{what}: lr {lr}")
     if total_norm is not None and not max_norm > 0.0:
@@ -141,7 +146,7 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32, or 8 for moments of 8 bits (2.06 bytes per weight instead
     of 8).  Weights in bf16 get an fp32 master in their state, which the update
     reads and writes; the weights are its rounding.  The step counts live
-    on the device, ``lr`` may be a device tensor: a step can be captured.
+    on the device, ``lr`` may be a device tensor (of a host tensor a captured step keeps the value): a step can be captured.
     With 32 bits the state is torch.optim.AdamW's, and either loads the other's.
 
     step(max_norm=...) clips the gradients by their norm over all groups as

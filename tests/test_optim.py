@@ -312,3 +312,13 @@ def test_lazy_clones_are_written_apart(emulated):
         lists[i][0] = torch._lazy_clone(original)
         optim.adamw_step(*lists, 1, **oc.HYPER)
         assert torch.equal(original, kept) and not torch.equal(lists[i][0], kept)
+
+
+def test_learning_rate_as_a_host_tensor():
+    """A number to weights on the device (the kernel could not read it), whatever its type; a device tensor is handed on."""
+    from gdino_amd import optim
+    lr, device = torch.tensor(0.25, dtype=torch.float64), torch.device("cuda", 0)
+    assert optim._learning_rate(lr, device) == (None, 0.25) and optim._learning_rate(0.25, device) == (None, 0.25)
+    assert optim._learning_rate(lr, lr.device) == (lr, 0.0)
+    there = torch.empty((), device="meta")
+    assert optim._learning_rate(there, device)[0] is there

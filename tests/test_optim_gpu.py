@@ -203,3 +203,21 @@ def test_optimizer_in_the_train_step():
         torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
         # each of 5 updates is at most about 1.2 lr; 8-bit moments are within 2^-3 of theirs
         assert torch.isfinite(c).all() and float((a - c).abs().max()) < 5 * 1.2e-3
+
+
+def test_learning_rate_as_a_host_tensor():
+    """AdamW(lr=torch.tensor(...)) on the host, as torch's schedulers write it, steps like the number."""
+    from gdino_amd import optim
+    sets = [torch.nn.Linear(40, 24).cuda() for _ in range(2)]
+    sets[1].load_state_dict(sets[0].state_dict())
+    lrs = torch.tensor(0.01, dtype=torch.float64), 0.01
+    opts = [optim.AdamW(net.parameters(), lr=lr) for net, lr in zip(sets, lrs)]
+    for t in range(3):
+        for net, opt in zip(sets, opts):
+            for p in net.parameters():
+                p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(t)).cuda()
+            opt.step(max_norm=0.5)
+        for a, b in zip(sets[0].parameters(), sets[1].parameters()):
+            assert torch.equal(a, b)
+        lrs[0].mul_(0.5)
+        opts[1].param_groups[0]["lr"] *= 0.5
