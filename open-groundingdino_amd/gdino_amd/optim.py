@@ -162,11 +162,30 @@ class AdamW(torch.optim.Optimizer):
         # capturable: what torch's loader asks before it moves a step count to the device
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       seed=seed, capturable=True))
-        for group in self.param_groups:
+        self.total_norm = None
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            self._check_options(group)
+            if group["state_bits"] not in (8, 32):
+                raise ValueError(f"state_bits {group['state_bits']}: 8 or 32")
             for p in group["params"]:
                 if p.dtype not in (torch.float32, torch.bfloat16):
                     raise TypeError(f"gdino_amd AdamW: unsupported dtype {p.dtype}")
-        self.total_norm = None
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_options(group):
+        """Options of torch's optimizers that change the update, and that this one lacks."""
+        for name in ("amsgrad", "maximize", "differentiable"):
+            if group.get(name):
+                raise ValueError(f"AdamW: {name} is not implemented")
+        if not group.get("decoupled_weight_decay", True) and group["weight_decay"] != 0:
+            raise ValueError("AdamW: the weight decay is decoupled from the gradient, not added to it")
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -234,6 +253,8 @@ class AdamW(torch.optim.Optimizer):
         return norms[0] if len(norms) == 1 else grad_norm(norms)
 
     def load_state_dict(self, state_dict):
+        for group in state_dict["param_groups"]:
+            self._check_options(group)
         bits = [g["state_bits"] for g in self.param_groups]
         seeds = [g["seed"] for g in self.param_groups]
         saved, at = {}, 0

@@ -322,3 +322,38 @@ def test_learning_rate_as_a_host_tensor():
     assert optim._learning_rate(lr, lr.device) == (lr, 0.0)
     there = torch.empty((), device="meta")
     assert optim._learning_rate(there, device)[0] is there
+
+
+def test_options_of_torch_that_are_not_implemented(emulated):
+    """A checkpoint or a group with amsgrad, maximize, differentiable or an L2 decay is refused, not stepped as if it had none."""
+    from gdino_amd import optim
+
+    def trained(cls=torch.optim.AdamW, **kw):
+        p = torch.ones(3, requires_grad=True)
+        p.grad = torch.ones(3)
+        opt = cls([p], lr=0.1, weight_decay=0.1, **kw)
+        opt.step()
+        return opt.state_dict()
+
+    def fresh():
+        return optim.AdamW([torch.ones(3, requires_grad=True)], lr=0.1)
+
+    for name in ("amsgrad", "maximize", "differentiable"):
+        saved = trained() if name == "differentiable" else trained(**{name: True})
+        saved["param_groups"][0][name] = True
+        opt = fresh()
+        with pytest.raises(ValueError, match=name):
+            opt.load_state_dict(saved)
+        assert not opt.state and name not in opt.param_groups[0]
+        with pytest.raises(ValueError, match=name):
+            optim.AdamW([{"params": [torch.ones(3, requires_grad=True)], name: True}])
+        with pytest.raises(ValueError, match=name):
+            opt.add_param_group({"params": [torch.ones(3, requires_grad=True)], name: True})
+        assert len(opt.param_groups) == 1
+    with pytest.raises(ValueError, match="decoupled"):
+        fresh().load_state_dict(trained(torch.optim.Adam))
+    fresh().load_state_dict(trained())
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        fresh().add_param_group({"params": [torch.ones(3, dtype=torch.float16, requires_grad=True)]})
+    with pytest.raises(ValueError, match="state_bits"):
+        fresh().add_param_group({"params": [torch.ones(3, requires_grad=True)], "state_bits": 16})
