@@ -205,13 +205,16 @@ class AdamW(torch.optim.Optimizer):
     def _lists(self, group):
         """{(weight type, gradient type, device): {"param": [...], "grad": [...], the state's keys}}."""
         lists = {}
+        eight = ("exp_avg_scale", "exp_avg_sq_scale") if group["state_bits"] == 8 else ()
         for p in group["params"]:
+            keys = ("step", "exp_avg", "exp_avg_sq", *eight, *(("master",) if p.dtype != torch.float32 else ()))
             g = p.grad
             if g is None:
                 continue
             if g.is_sparse:
                 raise RuntimeError("AdamW: sparse gradients are not supported")
-            row = {"param": p, "grad": g, **self._state(p, group["state_bits"])}
+            state = self._state(p, group["state_bits"])
+            row = {"param": p, "grad": g, **{k: state[k] for k in keys}}
             if not p.is_contiguous():  # (a channels_last weight: everything is walked in its memory's order)
                 order = _memory_order(p)
                 row = {k: t.detach().permute(order) if t.shape == p.shape and k != "step" else t
@@ -272,8 +275,12 @@ class AdamW(torch.optim.Optimizer):
             g["state_bits"], g["capturable"] = b, True
             g.setdefault("seed", s)
         for p, st in saved.items():
+            if st and p.dtype == torch.float32:
+                self.state[p].pop("master", None)  # (of a low-precision model's weight)
             # (torch's loader casts a state to its weight's type: bytes and masters keep theirs; moments are fp32)
             for k, v in st.items():
+                if k not in self.state[p]:
+                    continue
                 if k == "step":
                     self.state[p][k] = torch.as_tensor(v, dtype=torch.float32).to(p.device).clone()
                 elif torch.is_tensor(v):

@@ -357,3 +357,30 @@ def test_options_of_torch_that_are_not_implemented(emulated):
         fresh().add_param_group({"params": [torch.ones(3, dtype=torch.float16, requires_grad=True)]})
     with pytest.raises(ValueError, match="state_bits"):
         fresh().add_param_group({"params": [torch.ones(3, requires_grad=True)], "state_bits": 16})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_with_more_in_them(emulated, bits):
+    """A parameter without a state before one whose state holds something else too, and a low-precision model's
+    checkpoint (its masters belong to bf16 weights) in an fp32 one: the step takes what it knows."""
+    from gdino_amd import optim
+    nets = [torch.nn.Linear(4, 3, bias=False) for _ in range(2)]
+    params = [p for n in nets for p in n.parameters()]
+    opt = optim.AdamW(params, lr=0.1, state_bits=bits)
+    opt.state[params[1]] = dict(optim.adamw_state(params[1], bits), step=torch.zeros(()), note=torch.ones(3))
+    for p in params:
+        p.grad = torch.ones_like(p)
+    before = [p.detach().clone() for p in params]
+    opt.step()
+    for p, b in zip(params, before):
+        torch.testing.assert_close(p, b * (1 - 0.1 * 1e-2) - 0.1, rtol=1e-6, atol=1e-6)
+    low = torch.nn.Linear(4, 3, bias=False, dtype=torch.bfloat16)
+    saved = optim.AdamW(low.parameters(), lr=0.1, state_bits=bits)
+    low.weight.grad = torch.ones_like(low.weight)
+    saved.step()
+    net = torch.nn.Linear(4, 3, bias=False)
+    opt = optim.AdamW(net.parameters(), lr=0.1, state_bits=bits)
+    opt.load_state_dict(saved.state_dict())
+    net.weight.grad = torch.ones_like(net.weight)
+    opt.step()
+    assert "master" not in opt.state[net.weight] and int(opt.state[net.weight]["step"]) == 2
