@@ -192,10 +192,10 @@ class AdamW(torch.optim.Optimizer):
         self.__dict__.setdefault("total_norm", None)
 
     def _state(self, p, bits):
+        if bits == 8 and not p.is_contiguous():
+            raise ValueError("AdamW: 8-bit moments belong to contiguous weights (their scales go by memory)")
         st = self.state[p]
         if not st:
-            if bits == 8 and not p.is_contiguous():
-                raise ValueError("AdamW: 8-bit moments belong to contiguous weights (their scales go by memory)")
             st["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             st.update(adamw_state(p, bits))
             if p.dtype != torch.float32:
@@ -286,6 +286,8 @@ class AdamW(torch.optim.Optimizer):
                 elif torch.is_tensor(v):
                     dt = torch.float32 if v.is_floating_point() else v.dtype
                     like = p if v.shape == p.shape else v
-                    self.state[p][k] = torch.empty_like(like, dtype=dt, device=p.device, requires_grad=False).copy_(v)
+                    order = torch.preserve_format if v.is_floating_point() else torch.contiguous_format  # (bytes: their scales')
+                    self.state[p][k] = torch.empty_like(like, dtype=dt, device=p.device, requires_grad=False,
+                                                        memory_format=order).copy_(v)
             if st and p.dtype != torch.float32 and "master" not in st:
                 self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)

@@ -384,3 +384,44 @@ def test_states_with_more_in_them(emulated, bits):
     net.weight.grad = torch.ones_like(net.weight)
     opt.step()
     assert "master" not in opt.state[net.weight] and int(opt.state[net.weight]["step"]) == 2
+
+
+def test_eight_bit_checkpoint_of_another_memory_order(emulated):
+    """8-bit moments go by memory with their scales: a channels_last weight that has a checkpoint's, and one that became
+    channels_last, are refused at the step, with nothing changed; the checkpoint goes on to a contiguous one."""
+    from gdino_amd import optim
+
+    def conv(fmt):
+        torch.manual_seed(0)
+        return torch.nn.Conv2d(3, 4, 3, bias=False).to(memory_format=fmt)
+
+    def grads(net):
+        net.weight.grad = torch.ones_like(net.weight)
+
+    net = conv(torch.contiguous_format)
+    opt = optim.AdamW(net.parameters(), lr=0.1, state_bits=8)
+    grads(net)
+    opt.step()
+    other = conv(torch.channels_last)
+    assert not other.weight.is_contiguous()
+    again = optim.AdamW(other.parameters(), lr=0.1, state_bits=8)
+    again.load_state_dict(copy.deepcopy(opt.state_dict()))
+    grads(other)
+    with pytest.raises(ValueError, match="contiguous weights"):
+        again.step()
+    third = conv(torch.contiguous_format)
+    last = optim.AdamW(third.parameters(), lr=0.1, state_bits=8)
+    last.load_state_dict(copy.deepcopy(again.state_dict()))
+    third.load_state_dict(net.state_dict())
+    grads(third)
+    last.step()
+    opt.step()
+    assert torch.equal(net.weight, third.weight)
+    assert all(torch.equal(a, opt.state[net.weight][k]) for k, a in last.state[third.weight].items())
+    net.to(memory_format=torch.channels_last)
+    grads(net)
+    before, saved = net.weight.detach().clone(), copy.deepcopy(opt.state_dict()["state"])
+    with pytest.raises(ValueError, match="contiguous weights"):
+        opt.step()
+    assert torch.equal(net.weight, before)
+    assert all(torch.equal(a, b) for a, b in zip(opt.state_dict()["state"][0].values(), saved[0].values()))
