@@ -276,10 +276,16 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias, con
 }
 
 // -------------------------------------------------------------- lists of tensors
+struct Span {
+  uint64_t begin, end;
+  bool written;
+  bool operator<(const Span& o) const { return begin < o.begin; }
+};
 struct List {
   std::vector<Tensor> held;
   std::vector<uint64_t> at;
   std::vector<int64_t> size;
+  std::vector<Span> spans;  // of the tensors with elements, ascending
 };
 
 // the one or two types a list may have
@@ -302,7 +308,7 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
   out.held.reserve(n);
   out.at.resize(n);
   out.size.resize(n);
-  std::vector<std::pair<uint64_t, uint64_t>> spans;
+  out.spans.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = tuple ? PyTuple_GET_ITEM(list, i) : PyList_GET_ITEM(list, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": ", name, " ", i, " is not a tensor but ", Py_TYPE(o)->tp_name);
@@ -318,14 +324,33 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
     TORCH_CHECK_VALUE(!sizes || (*sizes)[i] == out.size[i], what, ": ", name, " and the weights differ in their numbers of elements");
     // (a tensor that is written stops sharing a lazy clone's memory first)
     out.at[i] = out.size[i] ? reinterpret_cast<uint64_t>(written ? t.mutable_data_ptr() : t.const_data_ptr()) : 0;
-    if (written && out.size[i]) spans.emplace_back(out.at[i], out.at[i] + uint64_t(out.size[i]) * t.element_size());
+    if (out.size[i]) out.spans.push_back({out.at[i], out.at[i] + uint64_t(out.size[i]) * t.element_size(), written});
     out.held.push_back(t);
   }
-  std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK_VALUE(spans[i].first >= spans[i - 1].second, what, ": ", name,
+  std::sort(out.spans.begin(), out.spans.end());
+  for (size_t i = 1; written && i < out.spans.size(); ++i)
+    TORCH_CHECK_VALUE(out.spans[i].begin >= out.spans[i - 1].end, what, ": ", name,
                       " overlap in memory (or a tensor is listed twice), and they are updated");
   return out;
+}
+
+// whether a written tensor of one list overlaps one of another
+bool overlap(std::initializer_list<const List*> lists) {
+  std::vector<Span> all;
+  size_t n = 0;
+  for (const List* l : lists) n += l->spans.size();
+  all.reserve(n);
+  for (const List* l : lists) {
+    const auto joined = all.insert(all.end(), l->spans.begin(), l->spans.end());
+    std::inplace_merge(all.begin(), joined, all.end());
+  }
+  uint64_t written = 0, any = 0;  // where what began so far ends
+  for (const Span& s : all) {
+    if (s.begin < (s.written ? any : written)) return true;
+    any = std::max(any, s.end);
+    if (s.written) written = std::max(written, s.end);
+  }
+  return false;
 }
 
 const float* scalar_of(const char* what, const char* name, const Tensor& t, const at::Device& device) {
@@ -441,7 +466,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
       ls = list_of(what, "steps", steps, {at::kFloat}, &device, false, &ones);
     }
     if (lp.held.empty()) Py_RETURN_NONE;
-    // (a list given twice; within a list any overlap is found above)
+    // (a list given twice)
     for (size_t i = 0; i < size->size(); ++i) {
       if ((*size)[i] == 0) continue;
       const uint64_t of[] = {lp.at[i], lg.at[i], lm.at[i], lv.at[i], eight ? lms.at[i] : 0, eight ? lvs.at[i] : 0,
@@ -450,6 +475,8 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
         for (int b = 0; b < a; ++b)
           TORCH_CHECK_VALUE(of[a] == 0 || of[a] != of[b], what, ": two lists share tensor ", i);
     }
+    TORCH_CHECK_VALUE(!overlap({&lp, &lg, &lm, &lv, &lms, &lvs, &lc}), what,
+                      ": two lists overlap in memory, and one is updated");
     const Tensor lrt = tensor_of(lr_dev), nt = tensor_of(norm);
     const float* lrp = lrt.defined() ? scalar_of(what, "lr", lrt, *device) : nullptr;
     const float* np = nt.defined() ? scalar_of(what, "total_norm", nt, *device) : nullptr;

@@ -425,3 +425,39 @@ def test_eight_bit_checkpoint_of_another_memory_order(emulated):
         opt.step()
     assert torch.equal(net.weight, before)
     assert all(torch.equal(a, b) for a, b in zip(opt.state_dict()["state"][0].values(), saved[0].values()))
+
+
+def test_lists_that_overlap_are_refused(emulated):
+    """In part, or at different places of their lists; gradients, which are read, may overlap each other."""
+    from gdino_amd import optim
+
+    def refused(lists, **kw):
+        kept = [[x.clone() for x in some] for some in lists]
+        with pytest.raises(ValueError, match="overlap"):
+            optim.adamw_step(*lists, 1, **kw, **oc.HYPER)
+        assert all(torch.equal(a, b) for x, y in zip(lists, kept) for a, b in zip(x, y))
+
+    for a in range(4):
+        for b in range(a):
+            lists = oc.make([8, 8, 24])
+            flat = torch.ones(15)
+            lists[a][0], lists[b][0] = flat[:8], flat[7:]
+            refused(lists)
+            lists = oc.make([8, 8, 24])
+            lists[a][1] = lists[b][0]
+            refused(lists)
+            lists = oc.make([8, 8, 24])
+            lists[a][1] = lists[b][2][8:16]
+            refused(lists)
+    p, g, m, v = oc.make([8, 8])
+    refused((p, g, m, v), copies=[torch.zeros(8).bfloat16(), m[1].view(torch.bfloat16)[4:12]])
+    s = [optim.adamw_state(x, 8) for x in oc.make([64, 64])[0]]
+    p, g, _, _ = oc.make([64, 64])
+    lists = {k: [x[k] for x in s] for k in s[0]}
+    lists["exp_avg_scale"][1] = lists["exp_avg_sq"][0][10:12]
+    refused((p, g, lists["exp_avg"], lists["exp_avg_sq"]), exp_avg_scales=lists["exp_avg_scale"],
+            exp_avg_sq_scales=lists["exp_avg_sq_scale"])
+    p, g, m, v = oc.make([8, 8])
+    optim.adamw_step(p, [g[0], g[0]], m, v, 1, **oc.HYPER)
+    flat = torch.ones(12)
+    optim.adamw_step(p, [flat[:8], flat[4:]], m, v, 2, **oc.HYPER)
