@@ -1333,7 +1333,8 @@ Plan plan_of(int M, int N, int r) {
     double chunk, alone, base;
   };
   constexpr Kind kinds[] = {{256, 256, 1.5, 1.5, 11.5}, {128, 512, 0.80, 0.67, 5.0}, {64, 768, 0.55, 0.40, 2.9}};
-  const int forced = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256)
+  const int asked = env_int("GD_LINEAR_TILE", 0);  // (A/B: 64, 128 or 256; another value is none)
+  const int forced = asked == 64 || asked == 128 || asked == 256 ? asked : 0;
   const int64_t chunks = div_up(r, kR);
   Plan p = {};
   double best = 1e30;

@@ -459,3 +459,14 @@ def test_saved_tensors(emulated, act, residual, k):
         assert saved == want, which
         got = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, dy)))
         lc.check(x, w, b, act, r, y, dy, [got.get(id(t)) for t in (x, w, b, r)])
+
+
+@pytest.mark.parametrize("tile", ["1", "96", "-64", "512", "x", ""])
+def test_unknown_tiles_choose_by_themselves(emulated, monkeypatch, tile):
+    """GD_LINEAR_TILE with another value than 64, 128 or 256 is as good as none."""
+    monkeypatch.delenv("GD_LINEAR_TILE", raising=False)
+    x, w, b, r, dy = lc.inputs(70, 600, 30, BF, True, F32, seed=3)
+    want = lc.run(x, w, b, "gelu", r, dy)
+    monkeypatch.setenv("GD_LINEAR_TILE", tile)
+    got = lc.run(x, w, b, "gelu", r, dy)
+    assert torch.equal(got[0], want[0]) and all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
