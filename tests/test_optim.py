@@ -461,3 +461,35 @@ def test_lists_that_overlap_are_refused(emulated):
     optim.adamw_step(p, [g[0], g[0]], m, v, 1, **oc.HYPER)
     flat = torch.ones(12)
     optim.adamw_step(p, [flat[:8], flat[4:]], m, v, 2, **oc.HYPER)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_warm_ups_of_a_step_graph_are_rolled_back(bits, dtype):
+    """Weights, masters, moments, scales and step counts return to where they were: before a first step and after one."""
+    from gdino_amd import optim
+    from gdino_amd.stepgraph import TrainStepGraph  # (declares entry points that the emulator has no twin of)
+
+    def make():
+        torch.manual_seed(1)
+        net = torch.nn.Sequential(torch.nn.Linear(5, 7), torch.nn.Linear(7, 3)).to(dtype)
+        return net, optim.AdamW(net.parameters(), lr=1e-2, state_bits=bits, seed=3)
+
+    with emu_product.emulated_product():
+        net, opt = make()
+        same, plain = make()
+        g = TrainStepGraph(net, None, opt, amp_dtype=None)
+        for seed in (1, 2, 3):
+            snap = g._snapshot()
+            for warm in (7, 8):
+                _grads(net, warm)
+                opt.step(max_norm=0.1)
+            g._restore(snap)
+            for n, o in ((net, opt), (same, plain)):
+                _grads(n, seed)
+                o.step(max_norm=0.1)
+            for p, q in zip(net.parameters(), same.parameters()):
+                assert torch.equal(p, q)
+                if plain.state[q]:
+                    assert opt.state[p].keys() == plain.state[q].keys()
+                    assert all(torch.equal(x, plain.state[q][k]) for k, x in opt.state[p].items())

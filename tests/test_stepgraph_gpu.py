@@ -436,3 +436,40 @@ def test_text_bucket_changes_only_rounding(amp):
     rows = sorted(((rel(g64[n], g1[n]), rel(g1b[n], g1[n]), n) for n in g1), reverse=True)
     bad = [r for r in rows if not r[0] <= max(floor, 5 * r[1])]
     assert g1.keys() == g64.keys() and not bad, (len(bad), bad[:8], rows[:8])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_hip_adamw_in_the_step_graph(bits):
+    """optim.AdamW inside the captured step (step counts and lr on the device, the clip folded in): two steps move the
+    weights as two eager ones do, and, with fp32 moments, as torch's AdamW with clip_grad_norm_ does."""
+    from gdino_amd import optim
+    from gdino_amd.config import make_args
+    from gdino_amd.stepgraph import TrainStepGraph
+    from gdino_amd.train import build_optimizer, train_step
+    b = _batch(21, 4)
+    upd, norms = {}, {}
+    for mode in ("torch", "eager", "eager2", "graph"):
+        model, crit, opt = _model()
+        if mode != "torch":
+            opt = build_optimizer(make_args(device=DEV, optimizer="adamw_hip", optimizer_state_bits=bits), model)
+            assert isinstance(opt, optim.AdamW)
+        p0 = _params(model)
+        if mode == "graph":
+            g = TrainStepGraph(model, crit, opt, warmup=2, text_multiple=1)
+            for _ in range(2):
+                g(*b)
+            assert g.stats()["mode"] == "graph" and g.stats()["captures"] == 1 and g.stats()["replays"] == 2
+        else:
+            for _ in range(2):
+                train_step(model, crit, opt, *b)
+        torch.cuda.synchronize()
+        upd[mode] = _params(model) - p0
+        assert {float(s["step"]) for s in opt.state.values()} == {2.0}, mode
+        if mode != "torch":
+            norms[mode] = float(opt.total_norm)
+    size = upd["eager"].norm()
+    noise = float((upd["eager2"] - upd["eager"]).norm() / size)
+    assert float((upd["graph"] - upd["eager"]).norm() / size) <= max(0.05, 3 * noise), noise
+    assert abs(norms["graph"] / norms["eager"] - 1) <= max(0.01, 3 * abs(norms["eager2"] / norms["eager"] - 1)), norms
+    if bits == 32:
+        assert float((upd["torch"] - upd["eager"]).norm() / size) <= max(0.05, 3 * noise), noise
