@@ -276,16 +276,12 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const Tensor& bias, con
 }
 
 // -------------------------------------------------------------- lists of tensors
-struct Span {
-  uint64_t begin, end;
-  bool written;
-  bool operator<(const Span& o) const { return begin < o.begin; }
-};
 struct List {
+  const char* name = "";
+  bool written = false;
   std::vector<Tensor> held;
   std::vector<uint64_t> at;
   std::vector<int64_t> size;
-  std::vector<Span> spans;  // of the tensors with elements, ascending
 };
 
 // the one or two types a list may have
@@ -296,7 +292,7 @@ struct Types {
 };
 
 // `list`: a list or tuple of contiguous tensors of one of `types`, alike, on one device (device: of the call, set by its
-// first list); written: not overlapping; sizes: the elements each has to have
+// first list); written: see require_apart; sizes: the elements each has to have
 List list_of(const char* what, const char* name, PyObject* list, Types types,
              std::optional<at::Device>* device, bool written, const std::vector<int64_t>* sizes) {
   const bool tuple = PyTuple_Check(list);
@@ -305,10 +301,11 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
   TORCH_CHECK_VALUE(!sizes || size_t(n) == sizes->size(), what, ": ", n, " ", name, " for ", sizes ? sizes->size() : 0,
                     " tensors");
   List out;
+  out.name = name;
+  out.written = written;
   out.held.reserve(n);
   out.at.resize(n);
   out.size.resize(n);
-  out.spans.reserve(n);
   for (Py_ssize_t i = 0; i < n; ++i) {
     PyObject* o = tuple ? PyTuple_GET_ITEM(list, i) : PyList_GET_ITEM(list, i);
     TORCH_CHECK_TYPE(THPVariable_Check(o), what, ": ", name, " ", i, " is not a tensor but ", Py_TYPE(o)->tp_name);
@@ -324,33 +321,39 @@ List list_of(const char* what, const char* name, PyObject* list, Types types,
     TORCH_CHECK_VALUE(!sizes || (*sizes)[i] == out.size[i], what, ": ", name, " and the weights differ in their numbers of elements");
     // (a tensor that is written stops sharing a lazy clone's memory first)
     out.at[i] = out.size[i] ? reinterpret_cast<uint64_t>(written ? t.mutable_data_ptr() : t.const_data_ptr()) : 0;
-    if (out.size[i]) out.spans.push_back({out.at[i], out.at[i] + uint64_t(out.size[i]) * t.element_size(), written});
     out.held.push_back(t);
   }
-  std::sort(out.spans.begin(), out.spans.end());
-  for (size_t i = 1; written && i < out.spans.size(); ++i)
-    TORCH_CHECK_VALUE(out.spans[i].begin >= out.spans[i - 1].end, what, ": ", name,
-                      " overlap in memory (or a tensor is listed twice), and they are updated");
   return out;
 }
 
-// whether a written tensor of one list overlaps one of another
-bool overlap(std::initializer_list<const List*> lists) {
-  std::vector<Span> all;
-  size_t n = 0;
-  for (const List* l : lists) n += l->spans.size();
-  all.reserve(n);
-  for (const List* l : lists) {
-    const auto joined = all.insert(all.end(), l->spans.begin(), l->spans.end());
-    std::inplace_merge(all.begin(), joined, all.end());
-  }
-  uint64_t written = 0, any = 0;  // where what began so far ends
+// What is written overlaps nothing: no tensor of its own list, and none of another (what is only read may overlap what is).
+void require_apart(const char* what, std::initializer_list<const List*> lists) {
+  struct Span {
+    uint64_t begin, end;
+    const List* list;
+  };
+  c10::SmallVector<const List*, 8> in_order(lists.begin(), lists.end());
+  // (lists that are cut from buffers one after the other need no sorting then)
+  const auto first = [](const List* l) { return l->at.empty() ? 0 : l->at[0]; };
+  std::sort(in_order.begin(), in_order.end(), [&](const List* a, const List* b) { return first(a) < first(b); });
+  c10::SmallVector<Span, 64> all;
+  for (const List* l : in_order)
+    for (size_t i = 0; i < l->at.size(); ++i)
+      if (l->size[i]) all.push_back({l->at[i], l->at[i] + uint64_t(l->size[i]) * l->held[i].element_size(), l});
+  const auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(all.begin(), all.end(), before)) std::sort(all.begin(), all.end(), before);
+  const Span *any = nullptr, *written = nullptr;  // what reaches furthest so far
   for (const Span& s : all) {
-    if (s.begin < (s.written ? any : written)) return true;
-    any = std::max(any, s.end);
-    if (s.written) written = std::max(written, s.end);
+    const Span* const other = s.list->written ? any : written;
+    if (other && s.begin < other->end) {
+      TORCH_CHECK_VALUE(other->list != s.list, what, ": ", s.list->name,
+                        " overlap in memory (or a tensor is listed twice), and they are updated");
+      TORCH_CHECK_VALUE(false, what, ": ", other->list->name, " and ", s.list->name,
+                        " overlap in memory, and one of them is updated");
+    }
+    if (!any || s.end > any->end) any = &s;
+    if (s.list->written && (!written || s.end > written->end)) written = &s;
   }
-  return false;
 }
 
 const float* scalar_of(const char* what, const char* name, const Tensor& t, const at::Device& device) {
@@ -466,7 +469,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
       ls = list_of(what, "steps", steps, {at::kFloat}, &device, false, &ones);
     }
     if (lp.held.empty()) Py_RETURN_NONE;
-    // (a list given twice)
+    // (a list given twice; the common mistake, named by its place)
     for (size_t i = 0; i < size->size(); ++i) {
       if ((*size)[i] == 0) continue;
       const uint64_t of[] = {lp.at[i], lg.at[i], lm.at[i], lv.at[i], eight ? lms.at[i] : 0, eight ? lvs.at[i] : 0,
@@ -475,8 +478,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* args) {
         for (int b = 0; b < a; ++b)
           TORCH_CHECK_VALUE(of[a] == 0 || of[a] != of[b], what, ": two lists share tensor ", i);
     }
-    TORCH_CHECK_VALUE(!overlap({&lp, &lg, &lm, &lv, &lms, &lvs, &lc}), what,
-                      ": two lists overlap in memory, and one is updated");
+    require_apart(what, {&lp, &lg, &lm, &lv, &lms, &lvs, &lc});
     const Tensor lrt = tensor_of(lr_dev), nt = tensor_of(norm);
     const float* lrp = lrt.defined() ? scalar_of(what, "lr", lrt, *device) : nullptr;
     const float* np = nt.defined() ? scalar_of(what, "total_norm", nt, *device) : nullptr;
