@@ -172,12 +172,10 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     // x for W's gradient, W for x's, z or y for the slope
     ctx->save_for_backward({weight.requires_grad() ? f.x : Tensor(), x.requires_grad() ? f.w : Tensor(),
                             !wants || act == 0 ? Tensor() : by_y ? f.y : f.z});
-    ctx->saved_data["act"] = act;
     ctx->saved_data["x"] = x.sizes().vec();
-    ctx->saved_data["of"] = std::vector<int64_t>{x2.size(0), weight.size(0)};
-    ctx->saved_data["types"] =
-        std::vector<int64_t>{int64_t(x.scalar_type()), int64_t(weight.scalar_type()), int64_t(xc.scalar_type())};
-    ctx->saved_data["given"] = std::vector<int64_t>{bias.has_value(), residual.has_value()};
+    ctx->saved_data["call"] =
+        std::vector<int64_t>{act, x2.size(0), weight.size(0), int64_t(x.scalar_type()), int64_t(weight.scalar_type()),
+                             int64_t(xc.scalar_type()), bias.has_value(), residual.has_value()};
     return f.y;
   }
 
@@ -189,14 +187,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear_act: gradients of its gradients are not implemented");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1];
-    const int act = int(ctx->saved_data["act"].toInt());
-    const auto given = ctx->saved_data["given"].toIntVector(), types = ctx->saved_data["types"].toIntVector();
+    const auto call = ctx->saved_data["call"].toIntVector(), shape = ctx->saved_data["x"].toIntVector();
+    const int act = int(call[0]);
+    const int64_t m = call[1], n = call[2], k = shape.back();
+    const auto xt = at::ScalarType(call[3]), wt = at::ScalarType(call[4]), type = at::ScalarType(call[5]);
+    const bool has_b = call[6], has_r = call[7];
     const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
-    const bool want_b = given[0] && ctx->needs_input_grad(2), want_r = given[1] && ctx->needs_input_grad(2 + given[0]);
-    const auto shape = ctx->saved_data["x"].toIntVector();
-    const auto of = ctx->saved_data["of"].toIntVector();
-    const int64_t m = of[0], k = shape.back(), n = of[1];
-    const auto xt = at::ScalarType(types[0]), wt = at::ScalarType(types[1]);
+    const bool want_b = has_b && ctx->needs_input_grad(2), want_r = has_r && ctx->needs_input_grad(2 + has_b);
     const auto like = dy.options().requires_grad(false);
     Tensor dx, dw, db;
     if (want_x) dx = at::empty({m, k}, like.dtype(xt));
@@ -214,13 +211,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       const Tensor ws = workspace(bytes, g);
       const auto pitch = [](const Tensor& t) { return t.defined() ? t.stride(0) : 0; };
       run("gd_linear_backward",
-          api.linear_backward(code_of(at::ScalarType(types[2])), act, data(g), code_of(g.scalar_type()), g.stride(0), data(z),
+          api.linear_backward(code_of(type), act, data(g), code_of(g.scalar_type()), g.stride(0), data(z),
                               pitch(z), data(x), pitch(x), data(w), pitch(w), m, k, n, mut(dx), code_of(xt), k, mut(dw),
                               mut(db), code_of(wt), 1, mut(ws), bytes, stream_of(g)));
     }
     if (want_x) out[0] = dx.view(shape);
     out[1] = dw;
-    if (given[0]) out[2] = db;
+    if (has_b) out[2] = db;
     if (want_r) out[3] = dy;
     return out;
   }
