@@ -184,6 +184,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     torch::autograd::variable_list out(8);
     const Tensor dy = grads[0];
     if (!dy.defined()) return out;
+    require_no_obstacle("linear_act's gradient", {&dy});
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear_act: gradients of its gradients are not implemented");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1];

@@ -470,3 +470,24 @@ def test_unknown_tiles_choose_by_themselves(emulated, monkeypatch, tile):
     monkeypatch.setenv("GD_LINEAR_TILE", tile)
     got = lc.run(x, w, b, "gelu", r, dy)
     assert torch.equal(got[0], want[0]) and all(torch.equal(a, c) for a, c in zip(got[1], want[1]))
+
+
+def test_gradients_of_tracing_and_transforms_are_refused(emulated):
+    """A backward pass alone under a trace, a dual dy, batched gradients: refused as the forward is."""
+    import torch.autograd.forward_ad as fwd
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from gdino_amd.linear import linear_act
+    x, w, b, _, dy = lc.inputs(6, 24, 16, BF)
+    y = linear_act(x, w, b, "gelu")
+
+    def grad(d, **kw):
+        return torch.autograd.grad(y, (x, w, b), d, retain_graph=True, **kw)
+
+    want = grad(dy)
+    with pytest.raises(RuntimeError, match="gradient: it cannot be traced"):
+        make_fx(grad)(dy)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="gradient: it has no forward-mode"):
+        grad(fwd.make_dual(dy, dy))
+    with pytest.raises(RuntimeError, match="gradient: it takes plain tensors"):
+        grad(dy[None], is_grads_batched=True)
+    assert all(torch.equal(a, c) for a, c in zip(grad(dy), want))
