@@ -136,12 +136,10 @@ __device__ __forceinline__ void activate8(float v[8], int act) {
   }
 }
 
-// Where the smooth slopes are 0 and 1 in fp32, z is taken as +-128: an infinite z (in fp16 any beyond 65504, whose
-// layer may well be finite with an fp32 residual) would make them inf * 0.  NaN stays.
-__device__ __forceinline__ float slope_arg(float z) {
-  z = z > 128.f ? 128.f : z;
-  return z < -128.f ? -128.f : z;
-}
+// z as a factor of a term that vanishes far from zero: an infinite one (in fp16 any beyond 65504, whose layer may well be
+// finite with an fp32 residual) would make it inf * 0.  From 128 on the smooth slopes are 0 and 1 in fp32; NaN stays, by
+// the other factors.
+__device__ __forceinline__ float slope_arg(float z) { return fminf(fmaxf(z, -128.f), 128.f); }
 
 // d[j] *= act'(z[j])
 __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
@@ -153,23 +151,22 @@ __device__ __forceinline__ void slope8(float d[8], const float z[8], int act) {
     case kGelu:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = slope_arg(z[j]);
         float bell;
-        const float c = normal_cdf(x, &bell);
-        d[j] *= c + x * bell * 0.39894228040143268f;
+        const float c = normal_cdf(z[j], &bell);
+        d[j] *= c + slope_arg(z[j]) * bell * 0.39894228040143268f;
       }
       break;
     case kGeluTanh:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = slope_arg(z[j]), q = tanh_gate(x);
+        const float x = slope_arg(z[j]), q = tanh_gate(z[j]);
         d[j] *= q + 2.f * x * q * (1.f - q) * kTanhC * (1.f + 3.f * kTanhA * x * x);
       }
       break;
     case kSilu:
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = slope_arg(z[j]), q = sigmoid(x);
+        const float x = slope_arg(z[j]), q = sigmoid(z[j]);
         d[j] *= q * (1.f + x * (1.f - q));
       }
       break;

@@ -201,3 +201,16 @@ def check_far_from_zero(device, act, dtype, size, residual, m=130, k=128, n=192)
     near(dx, dz @ w64, e @ w64.abs() + (n + 2) * U * (dz.abs() @ w64.abs()))
     near(dw, dz.t() @ x64, e.t() @ x64.abs() + (m + 2) * U * (dz.abs().t() @ x64.abs()))
     near(db, dz.sum(0), (m + 2) * U * dz.abs().sum(0) + 2.0 ** -25)
+
+
+def check_nan_slopes(device, act, m=70, k=24, n=64):
+    """A NaN z is a NaN slope: its row of dx, and db, have it; the other rows do not."""
+    from gdino_amd.linear import linear_act
+    x, w, b, _, dy = inputs(m, k, n, torch.float16, device=device, seed=3)
+    with torch.no_grad():
+        x[5, 1] = float("nan")
+    y = linear_act(x, w, b, act)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    rows = torch.ones(m, dtype=torch.bool, device=device)
+    rows[5] = False
+    assert torch.isnan(dx[5]).all() and torch.isfinite(dx[rows]).all() and torch.isnan(db).all() and torch.isnan(dw).all()

@@ -491,3 +491,10 @@ def test_gradients_of_tracing_and_transforms_are_refused(emulated):
     with pytest.raises(RuntimeError, match="gradient: it takes plain tensors"):
         grad(dy[None], is_grads_batched=True)
     assert all(torch.equal(a, c) for a, c in zip(grad(dy), want))
+
+
+@pytest.mark.parametrize("together", ["1", "1000000000"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_slopes_at_nan(emulated, monkeypatch, act, together):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_nan_slopes("cpu", act)

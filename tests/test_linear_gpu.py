@@ -267,3 +267,10 @@ def test_slopes_far_from_zero(monkeypatch, act, tile, together):
     lc.check_far_from_zero("cuda", act, HF, 90000.0, F32)
     lc.check_far_from_zero("cuda", act, HF, 90000.0, None)
     lc.check_far_from_zero("cuda", act, BF, 1e22, None)
+
+
+@pytest.mark.parametrize("together", ["1", "1000000000"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_slopes_at_nan(monkeypatch, act, together):
+    monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
+    lc.check_nan_slopes("cuda", act)
