@@ -215,8 +215,9 @@ __device__ __forceinline__ void ld8(const void* p, int64_t at, bool f32, bool ve
   for (int j = 0; j < 8; ++j) v[j] = E::up(w.h[j]);
 }
 
-// 16 bytes of an output, which nothing reads soon: past the caches' ways of lines that are kept
-// (16384 x 512 -> 4096: 112 us with plain stores, 102 with these; 44446 x 256 -> 2048: 108 and 98)
+// 16 bytes of an output: past the caches' ways of lines that are kept (16384 x 512 -> 4096: 112 us with plain stores, 102
+// with these; 44446 x 256 -> 2048: 108 and 98).  Measured as a call by itself: what a next layer that reads the output at
+// once pays for it is not in these figures.
 __device__ __forceinline__ void st_out(void* p, uint4 u) {
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   GD_STORE_NT((u32x4{u.x, u.y, u.z, u.w}), static_cast<u32x4*>(p));
@@ -1412,7 +1413,7 @@ Epi plain_epi(void* y, bool f32, int64_t ldy) {
   return e;
 }
 
-// workgroups along the rows of linear_dact: about 1024 in all, each of at least 32 rows per lane group
+// workgroups along the rows of linear_dact: about 1024 in all, each of at least 4 rows per lane group
 struct DactPlan {
   int lanes, slabs, blocks;
   int64_t rows;

@@ -280,6 +280,8 @@ __device__ __forceinline__ void adamw_four(const AdamTable<E8, CP, ST>& t, const
 
 // Measured: 62 M weights in 385 tensors with moments in 8 bits 185 us (5.4 TB/s); with fp32 moments and the norm 313 us, 400 M
 // fp32 masters with bf16 gradients and copies, 8 bits and the norm 1250 us (5.8 TB/s).  A copy of 1 GiB runs at 5.2 TB/s.
+// With the counts on the device (ST) 62 M weights take 285 us for 280 (no norm), in 8 bits 212 for 194: doubles in every
+// wave, and a table of 60 tensors for 68.
 template <typename TG, bool E8, bool CP, bool ST>
 __global__ void __launch_bounds__(kOpThreads)
 adamw_kernel(const AdamTable<E8, CP, ST> t, const AdamConst c) {
@@ -411,7 +413,8 @@ __device__ __forceinline__ double block_sum(double x, double* lds) {
   return r;
 }
 
-// Measured: 400 M fp32 values in 290 tensors 276 us (5.8 TB/s); eight loads under way, coarser or finer pieces: no faster.
+// Measured: 400 M fp32 values in 290 tensors 276 us when repeated (the last 256 MB stay in the
+// memory-side cache), 326 on gradients not read before (4.9 TB/s); eight loads under way, coarser or finer pieces: no faster.
 template <typename TG>
 __global__ void __launch_bounds__(kOpThreads) norm_chunk_kernel(const NormTable t) {
   __shared__ double lds[kOpThreads / 64];
@@ -456,8 +459,8 @@ __global__ void __launch_bounds__(kNormJoin) norm_join_kernel(const double* __re
   if (threadIdx.x == 0) *out = float(sqrt(s));
 }
 
-// Elements per workgroup: 4096 (latency: a few vector loads per lane) up to 2^24 elements in all, beyond that
-// a 4096th of them, so that the joining workgroup never reads more than a few values per thread.
+// Elements per workgroup: 4096 (latency: a few vector loads per lane) up to 2^25 elements in all, beyond that
+// an 8192nd of them, 2^22 at most, so that the joining workgroup reads some ten values per thread.
 int64_t norm_chunk(int64_t total) {
   const int64_t c = (total / 8192 + 1023) / 1024 * 1024;
   return c < 4096 ? 4096 : (c > (1 << 22) ? (1 << 22) : c);
