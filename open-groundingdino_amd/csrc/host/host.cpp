@@ -88,9 +88,12 @@ bool wrapped(const Tensor& t) {
 // hand on) has no memory to be read.
 const char* obstacle(std::initializer_list<const Tensor*> tensors) {
   using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  const bool modes = Modes::any_modes_set();
   if (at::tracer::impl::is_dispatch_enabled() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
-      (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
+      (modes && Modes::get_mode(Key::PROXY)))
     return "it cannot be traced (its kernels are not torch operations)";
+  if (modes && (Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL))) return kWrapped;  // (its outputs would be)
   const bool forward_mode = c10::AutogradState::get_tls_state().get_fw_grad_mode();
   for (const Tensor* t : tensors) {
     if (!t->defined()) continue;

@@ -391,8 +391,8 @@ def test_wrappers_are_refused_and_composed(emulated):
         with pytest.raises(RuntimeError, match="plain tensors"):
             linear.linear_act(fx, fw, fb)
         assert kernels.linear_act(fx, fw, fb).shape == (6, 16)
-        with pytest.raises(TypeError, match="gradients 0: .* plain tensors"):
-            optim.grad_norm([fx])
+    with pytest.raises(TypeError, match="gradients 0: .* plain tensors"):
+        optim.grad_norm([fx])
 
 
 def test_negated_views(emulated):
@@ -498,3 +498,20 @@ def test_gradients_of_tracing_and_transforms_are_refused(emulated):
 def test_slopes_at_nan(emulated, monkeypatch, act, together):
     monkeypatch.setenv("GD_LINEAR_TOGETHER", together)
     lc.check_nan_slopes("cpu", act)
+
+
+def test_plain_tensors_under_a_fake_mode_are_refused(emulated):
+    """The outputs that the call allocates would be wrappers."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from gdino_amd import linear, optim
+    x, w, b, _, _ = lc.inputs(6, 24, 16, BF, grad=False)
+    p = [torch.ones(8) for _ in range(4)]
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            linear.linear_act(x, w, b)
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            optim.grad_norm(p)
+        with pytest.raises(RuntimeError, match="plain tensors"):
+            optim.adamw_step(*([t] for t in p), 1, lr=1e-3)
+        assert not linear.supported(x, w, b)
+    assert all((t == 1).all() for t in p)
